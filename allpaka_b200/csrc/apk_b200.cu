@@ -1342,3 +1342,4 @@ int apk_dist_init(apk_ctx *c, int rank, int world, const void *unique_id) {
 #include "decode.inl"
 #include "noalloc.inl"
 #include "gguf.inl"
+#include "pages.inl"

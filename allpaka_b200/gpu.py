@@ -30,6 +30,10 @@ Q2_K = 10
 Q3_K = 11
 Q5_K = 13
 Q6_K = 14
+# element types of the paged cache and its rows
+F32 = 0
+F16 = 1
+BF16 = 30
 
 ACT_Q8, ACT_F32, ACT_AUTO = 0, 1, 2
 ATTN_IDENTITY = 1
@@ -108,6 +112,36 @@ class _BenchReq(C.Structure):
                 ("ffn", C.c_void_p), ("act_mode", C.c_uint32)]
 
 
+class _Pages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("ty", C.c_uint32), ("n_layers", C.c_uint32),
+                ("n_pages", C.c_uint32), ("page", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("k_stride", C.c_uint64 * 4), ("v_stride", C.c_uint64 * 4), ("table", C.c_void_p),
+                ("table_stride", C.c_uint64), ("n_seqs", C.c_uint32), ("width", C.c_uint32), ("lens", C.c_void_p),
+                ("refs", C.c_void_p), ("work", C.c_void_p)]
+
+
+class _Rope(C.Structure):
+    _fields_ = [("rot_dim", C.c_uint32), ("layout", C.c_uint32), ("scaling", C.c_uint32), ("base", C.c_float),
+                ("factor", C.c_float), ("attn_factor", C.c_float), ("beta_fast", C.c_float), ("beta_slow", C.c_float),
+                ("orig_ctx", C.c_uint32), ("freq_factors", C.c_void_p)]
+
+
+class _RopeReq(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("layer", C.c_uint32), ("rope", C.c_void_p), ("ty", C.c_uint32), ("q", C.c_void_p),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p), ("out_ty", C.c_uint32),
+                ("q_stride", C.c_uint64 * 2), ("k_stride", C.c_uint64 * 2), ("v_stride", C.c_uint64 * 2),
+                ("out_stride", C.c_uint64 * 2), ("n_heads", C.c_uint32), ("n_rows", C.c_uint32), ("cu", C.c_void_p),
+                ("seqs", C.c_void_p), ("n", C.c_uint32), ("positions", C.c_void_p), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p), ("eps", C.c_float)]
+
+
+class _AttendReq(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("layer", C.c_uint32), ("ty", C.c_uint32), ("q", C.c_void_p), ("out", C.c_void_p),
+                ("q_stride", C.c_uint64 * 2), ("out_stride", C.c_uint64 * 2), ("n_heads", C.c_uint32),
+                ("n_rows", C.c_uint32), ("cu", C.c_void_p), ("seqs", C.c_void_p), ("n", C.c_uint32), ("scale", C.c_float),
+                ("causal", C.c_int), ("window", C.c_uint32), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
 class _Stats(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in
                 ("calls", "launches", "encode_ns", "wait_ns", "weight_bytes",
@@ -127,6 +161,8 @@ EXPORTS = (
     "apk_kv_create", "apk_kv_destroy", "apk_kv_read", "apk_kv_write", "apk_attend", "apk_bench_attend",
     "apk_gguf_open", "apk_gguf_close", "apk_gguf_n_tensors", "apk_gguf_tensor_at", "apk_gguf_find",
     "apk_gguf_architecture", "apk_gguf_meta_u32", "apk_gguf_meta_f32", "apk_gguf_meta_str", "apk_gguf_mapping",
+    "apk_rope_append", "apk_attend_pages", "apk_attend_pages_ws", "apk_pages_reserve", "apk_pages_fork",
+    "apk_pages_release", "apk_pages_compact",
     "apk_model_open", "apk_model_get_info", "apk_model_token_req", "apk_model_attach", "apk_model_close",
 )
 
@@ -195,6 +231,14 @@ def load_library() -> C.CDLL:
     l.apk_dist_p2p_open.argtypes = [C.c_void_p, C.c_void_p]
     l.apk_dist_unique_id.argtypes = [C.c_void_p]
     l.apk_dist_init.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_void_p]
+    l.apk_rope_append.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int]
+    l.apk_attend_pages.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int]
+    l.apk_attend_pages_ws.argtypes = [C.c_void_p, C.c_void_p]
+    l.apk_attend_pages_ws.restype = C.c_size_t
+    l.apk_pages_reserve.argtypes = [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int]
+    l.apk_pages_fork.argtypes = [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]
+    l.apk_pages_release.argtypes = [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]
+    l.apk_pages_compact.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
     _lib = l
     return l
 
@@ -320,6 +364,116 @@ class KvCache:
         self._h = None
 
 
+# Device tensors (torch's, or anything with the same data_ptr / shape / stride / dtype / device) of the paged cache.
+_TENSOR_TY = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+
+
+def _tensor(t, what: str, shape, dtype: Optional[str], device: int, dense: bool = True):
+    """Checks one device tensor argument: its device, dimensions (None: any size) and type; dense = C-contiguous."""
+    if t.device.type != "cuda" or t.device.index != device:
+        raise ValueError(f"{what} is on {t.device}, the context on cuda:{device}")
+    if len(t.shape) != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape)):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple('*' if w is None else w for w in shape)}")
+    if dtype is not None and str(t.dtype) != dtype:
+        raise ValueError(f"{what} is {t.dtype}, expected {dtype}")
+    if dense and not t.is_contiguous():
+        raise ValueError(f"{what} is not contiguous")
+    return t
+
+
+def _rows(t, what: str, shape, device: int):
+    """Rows of heads: any strides between rows and heads, the dimensions of a head next to one another."""
+    _tensor(t, what, shape, None, device, dense=False)
+    if str(t.dtype) not in _TENSOR_TY:
+        raise ValueError(f"{what} is {t.dtype}, expected float32, float16 or bfloat16")
+    if t.stride(2) != 1:
+        raise ValueError(f"{what}: the dimensions of a head are not contiguous")
+    return _TENSOR_TY[str(t.dtype)], (C.c_uint64 * 2)(t.stride(0), t.stride(1))
+
+
+def _stream(stream, t) -> int:
+    """The cudaStream_t to work on: the caller's, or the current stream of the tensors' framework."""
+    if stream is not None:
+        return int(stream)
+    import torch
+
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _list32(a) -> np.ndarray:
+    a = np.asarray(a)
+    if a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31):
+        raise ValueError("sequence numbers and counts are 32-bit integers")
+    return np.ascontiguousarray(a.reshape(-1), dtype=np.int32)
+
+
+@dataclass
+class Rope:
+    """Rotary positions (``apk_rope``): ``dim`` of a head's dimensions turn, as ``"half"`` pairs (i, i + dim/2) or as
+    neighbouring ``"pairs"`` (2i, 2i + 1); ``scaling`` "none", "linear" or "yarn" stretches them over a longer context.
+    The frequencies are in the C header."""
+    dim: int
+    layout: str = "half"
+    base: float = 10000.0
+    scaling: str = "none"
+    factor: float = 1.0
+    orig_ctx: int = 0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attn_factor: float = 1.0
+    freq_factors: Optional[Sequence[float]] = None
+
+    def __post_init__(self):
+        if self.layout not in ("half", "pairs") or self.scaling not in ("none", "linear", "yarn"):
+            raise ValueError(f"layout {self.layout!r}, scaling {self.scaling!r}")
+        self._ff = None
+        if self.freq_factors is not None:
+            self._ff = _f32(self.freq_factors).reshape(-1)
+            if self._ff.size != self.dim // 2:
+                raise ValueError(f"{self._ff.size} frequency factors, expected {self.dim // 2}")
+        self._c = _Rope(self.dim, ("half", "pairs").index(self.layout), ("none", "linear", "yarn").index(self.scaling), self.base,
+                        self.factor, self.attn_factor, self.beta_fast, self.beta_slow, self.orig_ctx, _ptr(self._ff))
+
+
+class KvPages:
+    """A pool of KV pages for many sequences (``apk_pages``), in the caller's own device tensors:
+
+    ``k``, ``v``    [n_layers, n_pages, page, n_kv_heads, head_dim] float16 or bfloat16, any order of the first four axes
+                    in memory
+    ``table``       [n_seqs, width] int32: the pages of each sequence's positions, in order
+    ``lens``        [n_seqs] int32: positions of each sequence
+    ``refs``        [n_pages] int32: sequences that hold the page; 0 = free
+
+    An empty pool has zeros in ``lens`` and ``refs``.  The pool keeps the tensors alive; :meth:`Gpu.pages_reserve` and its
+    companions change them in place, in the order of the stream they are given."""
+
+    def __init__(self, gpu: "Gpu", k, v, table, lens, refs):
+        dev = gpu.device
+        _tensor(k, "k", (None,) * 5, None, dev, dense=False)
+        L, NP, page, H, D = k.shape
+        _tensor(v, "v", (L, NP, page, H, D), str(k.dtype), dev, dense=False)
+        if str(k.dtype) not in ("torch.float16", "torch.bfloat16"):
+            raise ValueError(f"pages of {k.dtype}, expected float16 or bfloat16")
+        if k.stride(4) != 1 or v.stride(4) != 1:
+            raise ValueError("the dimensions of a head are not contiguous")
+        _tensor(table, "table", (None, None), "torch.int32", dev, dense=False)
+        S, W = table.shape
+        if W > 1 and table.stride(1) != 1:
+            raise ValueError("the rows of the page table are not contiguous")
+        _tensor(lens, "lens", (S,), "torch.int32", dev)
+        _tensor(refs, "refs", (NP,), "torch.int32", dev)
+        self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
+        self.n_layers, self.n_pages, self.page, self.n_kv_heads, self.head_dim = L, NP, page, H, D
+        self.device, self.n_seqs, self.width = dev, S, W
+        self.work = refs.new_zeros(64 + 4 * S + 3 * NP)
+        #: what the last :meth:`Gpu.pages_reserve` reported, on the device: 0, the pages that were missing, or -1
+        self.short_by = self.work[0]
+        self._c = _Pages(k.data_ptr(), v.data_ptr(), _TENSOR_TY[str(k.dtype)], L, NP, page, H, D,
+                         (C.c_uint64 * 4)(*k.stride()[:4]), (C.c_uint64 * 4)(*v.stride()[:4]), table.data_ptr(),
+                         max(table.stride(0), W), S, W, lens.data_ptr(), refs.data_ptr(), self.work.data_ptr())
+        self._p = C.addressof(self._c)
+
+
 class Gpu:
     """One GPU context.  The module-level functions below forward to a
     process-wide instance, like the reference's lazily-initialised singleton
@@ -332,6 +486,7 @@ class Gpu:
         if rc != 0:
             raise GpuError(rc, self._l.apk_last_error(None).decode())
         self._h = h
+        self._device = device
         self._attached = []   # keeps attached buffers alive
         self._token_cache = {}
 
@@ -345,6 +500,15 @@ class Gpu:
             self.close()
         except Exception:
             pass
+
+    @property
+    def device(self) -> int:
+        """The CUDA device of this context (``apk_init``: a negative one picks LOCAL_RANK or 0)."""
+        if self._device < 0:
+            import torch
+
+            self._device = int(os.environ.get("LOCAL_RANK", "0")) % max(1, torch.cuda.device_count())
+        return self._device
 
     # -- status handling ---------------------------------------------------
     def _err(self) -> str:
@@ -569,6 +733,106 @@ class Gpu:
         if rc < 0:
             raise GpuError(rc, self._err())
         return ms.value
+
+    # -- paged KV cache ----------------------------------------------------------
+    # True = issued, False = declined (see ``last_decline``).  ``stream`` is a cudaStream_t handle; None takes the current
+    # stream of the tensors' device.  Nothing synchronises unless ``wait`` is set.
+    def _batch(self, pages: KvPages, layer: int, cu, seqs):
+        if pages.device != self.device:
+            raise ValueError(f"the pool is on cuda:{pages.device}, the context on cuda:{self.device}")
+        if not 0 <= layer < pages.n_layers:
+            raise ValueError(f"layer {layer} of {pages.n_layers}")
+        n = _tensor(cu, "cu", (None,), "torch.int32", self.device).shape[0] - 1
+        if n < 0:
+            raise ValueError("cu holds n + 1 row offsets")
+        if seqs is not None:
+            _tensor(seqs, "seqs", (n,), "torch.int32", self.device)
+        return n
+
+    def rope_append(self, pages: KvPages, layer: int, q, k, v, cu, rope: Optional[Rope], out=None, seqs=None, positions=None,
+                    q_norm=None, k_norm=None, eps: float = 1e-6, stream: Optional[int] = None, wait: bool = False) -> bool:
+        """``apk_rope_append``: per-head norms and rotation of one layer's new rows; q goes to ``out`` (None: in place),
+        k and v into the pages.  q [rows, heads, head_dim] (or None), k, v [rows, kv heads, head_dim]; rows
+        ``cu[i]`` .. ``cu[i+1]-1`` are the last positions of sequence ``seqs[i]`` (None: i)."""
+        n, dev, D = self._batch(pages, layer, cu, seqs), self.device, pages.head_dim
+        ty, ks = _rows(k, "k", (None, pages.n_kv_heads, D), dev)
+        T = k.shape[0]
+        vty, vs = _rows(v, "v", (T, pages.n_kv_heads, D), dev)
+        qty, qs = (ty, (C.c_uint64 * 2)()) if q is None else _rows(q, "q", (T, None, D), dev)
+        if vty != ty or qty != ty:
+            raise ValueError("q, k and v are of one type")
+        out = q if out is None else out
+        oty, os_ = (ty, (C.c_uint64 * 2)()) if q is None else _rows(out, "out", tuple(q.shape), dev)
+        if positions is not None:
+            _tensor(positions, "positions", (T,), "torch.int32", dev)
+        for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            if w is not None:
+                _tensor(w, what, (D,), "torch.float32", dev)
+        req = _RopeReq(pages._p, layer, None if rope is None else C.addressof(rope._c), ty,
+                       None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), None if q is None else out.data_ptr(), oty,
+                       qs, ks, vs, os_, 0 if q is None else q.shape[1], T, cu.data_ptr(),
+                       None if seqs is None else seqs.data_ptr(), n, None if positions is None else positions.data_ptr(),
+                       None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps)
+        return self._check(self._l.apk_rope_append(self._h, C.byref(req), _stream(stream, k), 1 if wait else 0))
+
+    def attend_pages(self, pages: KvPages, layer: int, q, cu, scale: float, out, seqs=None, causal: bool = True, window: int = 0,
+                     workspace=None, stream: Optional[int] = None, wait: bool = False) -> bool:
+        """``apk_attend_pages``: the batch's rows q [rows, heads, head_dim] over one layer of the pages, into ``out``; rows
+        ``cu[i]`` .. ``cu[i+1]-1`` are the last positions of sequence ``seqs[i]`` (None: i).  ``workspace``: a uint8 tensor of
+        ``apk_attend_pages_ws`` bytes, for this call alone while it runs; None takes one from the tensors' allocator."""
+        n, D = self._batch(pages, layer, cu, seqs), pages.head_dim
+        ty, qs = _rows(q, "q", (None, None, D), self.device)
+        oty, os_ = _rows(out, "out", tuple(q.shape), self.device)
+        if oty != ty:
+            raise ValueError("out is of q's type")
+        if window < 0:
+            raise ValueError(f"a window of {window}")
+        req = _AttendReq(pages._p, layer, ty, q.data_ptr(), out.data_ptr(), qs, os_, q.shape[1], q.shape[0], cu.data_ptr(),
+                         None if seqs is None else seqs.data_ptr(), n, scale, 1 if causal else 0, window, None, 0)
+        need = self._l.apk_attend_pages_ws(self._h, C.byref(req))
+        if need:
+            if workspace is None:
+                workspace = pages.work.new_empty((need + 3) // 4)
+            elif workspace.device != q.device:
+                raise ValueError(f"workspace is on {workspace.device}")
+            req.ws, req.ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        return self._check(self._l.apk_attend_pages(self._h, C.byref(req), _stream(stream, q), 1 if wait else 0))
+
+    def pages_reserve(self, pages: KvPages, seqs, n_new, stream: Optional[int] = None, wait: bool = True) -> bool:
+        """``apk_pages_reserve``: room for ``n_new[i]`` more positions in sequence ``seqs[i]`` (host lists).  False when pages are
+        missing or a row of the table is too short, and then nothing has changed; with ``wait`` off ``pages.short_by`` says so."""
+        a, b = self._lists(pages, seqs, n_new)
+        return self._check(self._l.apk_pages_reserve(self._h, pages._p, a.size, a.ctypes.data, b.ctypes.data,
+                                                     _stream(stream, pages.work), 1 if wait else 0))
+
+    def pages_fork(self, pages: KvPages, src, dst, stream: Optional[int] = None) -> bool:
+        """``apk_pages_fork``: sequence ``dst[i]`` becomes a second holder of ``src[i]``'s positions (host lists)."""
+        a, b = self._lists(pages, src, dst)
+        return self._check(self._l.apk_pages_fork(self._h, pages._p, a.size, a.ctypes.data, b.ctypes.data,
+                                                  _stream(stream, pages.work)))
+
+    def pages_release(self, pages: KvPages, seqs, keep, stream: Optional[int] = None) -> bool:
+        """``apk_pages_release``: sequence ``seqs[i]`` keeps its first ``keep[i]`` positions (host lists)."""
+        a, b = self._lists(pages, seqs, keep)
+        return self._check(self._l.apk_pages_release(self._h, pages._p, a.size, a.ctypes.data, b.ctypes.data,
+                                                     _stream(stream, pages.work)))
+
+    def pages_compact(self, pages: KvPages, page_map=None, stream: Optional[int] = None) -> bool:
+        """``apk_pages_compact``: the pages in use move to the lowest numbers; ``page_map`` [n_pages] int32 receives each page's
+        new number, -1 for a free one."""
+        self._lists(pages, (), ())
+        if page_map is not None:
+            _tensor(page_map, "page_map", (pages.n_pages,), "torch.int32", self.device)
+        return self._check(self._l.apk_pages_compact(self._h, pages._p, None if page_map is None else page_map.data_ptr(),
+                                                     _stream(stream, pages.work)))
+
+    def _lists(self, pages: KvPages, a, b):
+        if pages.device != self.device:
+            raise ValueError(f"the pool is on cuda:{pages.device}, the context on cuda:{self.device}")
+        a, b = _list32(a), _list32(b)
+        if a.size != b.size:
+            raise ValueError(f"lists of {a.size} and {b.size} entries")
+        return a, b
 
     # -- parity instrumentation ----------------------------------------------
     def debug_block_dots(self, ty, w, n_in, n_out, x, m=1):

@@ -50,6 +50,8 @@ extern "C" {
 #define APK_ERR_OOM (-5)
 
 /* GGML type ids (crates/allpaka-dtype/src/lib.rs:61-75). */
+#define APK_TY_F32 0u
+#define APK_TY_F16 1u
 #define APK_TY_Q5_0 6u
 #define APK_TY_Q8_0 8u
 #define APK_TY_Q2_K 10u
@@ -57,6 +59,7 @@ extern "C" {
 #define APK_TY_Q4_K 12u
 #define APK_TY_Q5_K 13u
 #define APK_TY_Q6_K 14u
+#define APK_TY_BF16 30u
 
 /* How activations meet the integer weights.  The reference picks this by call
  * site, not by dtype (crates/allpaka-backend/src/quantmat/mod.rs):
@@ -396,6 +399,137 @@ int apk_bench_attend(apk_ctx *ctx, const apk_kv *kv, const float *q, uint32_t m,
                      uint32_t reps, float *us_per_layer);
 
 void apk_stats(apk_ctx *ctx, apk_stats_t *out);
+
+/* ---- paged KV cache -------------------------------------------------------
+ * Many sequences in one pool of pages: the serving form of the cache above (the reference keeps one
+ * contiguous cache a session, crates/allpaka-model/src/kv.rs, and reuses prefixes on the host,
+ * prefix_cache.rs).  A step of a serving loop is
+ *     apk_pages_reserve                           once: room for the step's new positions
+ *     apk_rope_append, apk_attend_pages           per layer
+ *     apk_pages_fork / _release / _compact        between steps, as sequences branch and end
+ *
+ * All memory is the caller's DEVICE memory and all work goes to the caller's stream, in its order; no
+ * call allocates or synchronises (but with wait != 0), so each can be captured into a CUDA graph: the
+ * lengths, the page table and the batch are read by the kernels, the lists of _reserve, _fork and
+ * _release are part of the captured launch.  Calls that change one pool (and calls that read it
+ * meanwhile) are ordered by the caller; calls on different pools are independent of one another.
+ *
+ * Nothing that the device arrays hold can lead outside the buffers: a page number outside the pool is
+ * a page that is not there (its positions are not visible, stores to it are dropped), a length is cut
+ * to the row of the table, a sequence number outside the table has no positions, row offsets are cut to
+ * n_rows. */
+#define APK_PAGES_MAX_LIST 1024u  /* sequences one _reserve, _fork or _release names */
+#define APK_PAGES_MAX_BATCH 4096u /* sequences of one _rope_append or _attend */
+/* int32 values of apk_pages.work, the pool's scratch: zeroed by the caller once, then left alone */
+#define APK_PAGES_WORK(n_pages, n_seqs) (64u + 4u * (n_seqs) + 3u * (n_pages))
+typedef struct {
+    void *k, *v;              /* element (layer, page, position, kv head, dim); dims are contiguous, the start 16-byte aligned */
+    uint32_t ty;              /* APK_TY_F16 or APK_TY_BF16 */
+    uint32_t n_layers, n_pages;
+    uint32_t page;            /* positions a page, a power of two from 8 to 256 */
+    uint32_t n_kv_heads, head_dim; /* head_dim a multiple of 8 up to 256 */
+    uint64_t k_stride[4], v_stride[4]; /* elements between layers, pages, positions, kv heads: multiples of 8, any order */
+    int32_t *table;           /* [n_seqs][width]: the pages of each sequence's positions, in order */
+    uint64_t table_stride;    /* elements between rows, >= width */
+    uint32_t n_seqs, width;
+    int32_t *lens;            /* [n_seqs]: positions of each sequence */
+    int32_t *refs;            /* [n_pages]: sequences that hold the page; 0 = free */
+    int32_t *work;            /* APK_PAGES_WORK(n_pages, n_seqs) values; work[0] is what _reserve reports */
+} apk_pages;
+
+/* Room for n_new[i] more positions in sequence seqs[i]: its length grows, pages are taken from the
+ * free ones, lowest number first, in the order of the list.  A sequence that would write into a last
+ * page which others hold too first gets a copy of that page's positions (all layers); of several such
+ * sequences in one list the last keeps the original if nobody else holds it.  All or nothing: work[0]
+ * becomes 0, or the number of missing pages, or -1 when a row of the table is too short, and then
+ * nothing has changed.  wait != 0 synchronises the stream and declines with APK_DECLINE_INVALID_STATE
+ * in the last two cases.  seqs and n_new are HOST arrays; a sequence may be named once. */
+int apk_pages_reserve(apk_ctx *ctx, const apk_pages *pages, uint32_t n, const int32_t *seqs, const int32_t *n_new, void *stream,
+                      int wait);
+/* Sequence dst[i] becomes a second holder of src[i]'s positions, in place of what it held.  No page is
+ * copied: _reserve does that where one of them goes on writing.  HOST arrays; a destination may be
+ * named once and not as a source too. */
+int apk_pages_fork(apk_ctx *ctx, const apk_pages *pages, uint32_t n, const int32_t *src, const int32_t *dst, void *stream);
+/* Sequence seqs[i] keeps its first keep[i] positions (0: it ends); pages that nobody else holds become
+ * free.  HOST arrays; a sequence may be named once. */
+int apk_pages_release(apk_ctx *ctx, const apk_pages *pages, uint32_t n, const int32_t *seqs, const int32_t *keep, void *stream);
+/* Moves the pages in use (refs > 0) to the lowest numbers: with L of them, those numbered L and above
+ * move into the free ones below, both in ascending order; table and refs follow.  page_map, a device
+ * array [n_pages] or NULL, receives each page's new number, -1 for a free one. */
+int apk_pages_compact(apk_ctx *ctx, const apk_pages *pages, int32_t *page_map, void *stream);
+
+/* Rotary positions.  Pair i of rot_dim/2 turns by position * f_i radians, f_i = base^(-2i/rot_dim),
+ * divided by freq_factors[i] if given; LINEAR: divided by `factor`; YARN (arXiv:2309.00071):
+ * f_i/factor * r_i + f_i * (1 - r_i) with r_i = clamp((i - lo) / max(hi - lo, 0.001), 0, 1),
+ * lo = max(0, floor(c(beta_fast))), hi = min(rot_dim - 1, ceil(c(beta_slow))),
+ * c(b) = rot_dim ln(orig_ctx / (2 pi b)) / (2 ln base).  Sine and cosine are multiplied by attn_factor,
+ * and for YARN with factor > 1 by 0.1 ln(factor) + 1 as well.  Angles are formed in 64 bits. */
+#define APK_ROPE_HALF 0u  /* pair (i, i + rot_dim/2): NeoX, as apk_attn_in */
+#define APK_ROPE_PAIRS 1u /* pair (2i, 2i + 1) */
+#define APK_ROPE_NONE 0u
+#define APK_ROPE_LINEAR 1u
+#define APK_ROPE_YARN 2u
+typedef struct {
+    uint32_t rot_dim;  /* even, <= head_dim; the dimensions behind it pass through.  0: nothing is rotated */
+    uint32_t layout, scaling;
+    float base, factor, attn_factor, beta_fast, beta_slow;
+    uint32_t orig_ctx;
+    const float *freq_factors; /* HOST, rot_dim/2 values, or NULL */
+} apk_rope;
+
+/* One layer's new rows: per-head RMSNorm where a weight is given (x / sqrt(mean x^2 + eps) * w), then the
+ * rotation, of q and k, as in apk_attn_in; q goes to `out`, k and v (not rotated) into the pages, each
+ * rounded once.  Rows cu[i] .. cu[i+1]-1 are the LAST positions of sequence seqs[i] (its length counts
+ * them already: apk_pages_reserve): row cu[i] + j stands at position lens - rows + j.  It turns by
+ * that position, or by positions[row] if given.  Rows that belong to no sequence are left alone.
+ * A sequence may be named once. */
+typedef struct {
+    const apk_pages *pages;
+    uint32_t layer;
+    const apk_rope *rope;     /* NULL: nothing is rotated */
+    uint32_t ty;              /* of q, k and v: APK_TY_F32, _F16 or _BF16 */
+    const void *q;            /* n_rows x n_heads x head_dim, or NULL: k and v only */
+    const void *k, *v;        /* n_rows x n_kv_heads x head_dim */
+    void *out;                /* like q, of type out_ty; may be q itself */
+    uint32_t out_ty;
+    uint64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2]; /* elements between rows, heads: whole 16 bytes */
+    uint32_t n_heads, n_rows;
+    const int32_t *cu;        /* device, n + 1 row offsets */
+    const int32_t *seqs;      /* device, n sequence numbers, or NULL: 0 .. n-1 */
+    uint32_t n;
+    const int32_t *positions; /* device, n_rows, or NULL */
+    const float *q_norm, *k_norm; /* device, head_dim, or NULL */
+    float eps;
+} apk_rope_req;
+int apk_rope_append(apk_ctx *ctx, const apk_rope_req *req, void *stream, int wait);
+
+/* Attention of the batch's rows over one layer of the pages (apk_attend's for many sequences and for
+ * chunks of any number of rows): row j of a sequence, at position p = lens - rows + j, gets
+ * sum_i softmax_i(scale * q.k_i) v_i over the positions i < lens with i <= p (causal != 0) and i > p - window
+ * (window != 0); GQA group = n_heads / n_kv_heads <= 64, head_dim 64 or 128.  A row that sees no position
+ * becomes zeros; rows that belong to no sequence are left alone.  What invisible positions hold
+ * (infinities, NaN) does not matter.  Rows are of the pages' type, or f32 over f16 pages. */
+typedef struct {
+    const apk_pages *pages;
+    uint32_t layer;
+    uint32_t ty;              /* of q and out */
+    const void *q;            /* n_rows x n_heads x head_dim */
+    void *out;                /* like q; not overlapping it */
+    uint64_t q_stride[2], out_stride[2]; /* elements between rows, heads: whole 16 bytes */
+    uint32_t n_heads, n_rows;
+    const int32_t *cu, *seqs; /* device, as in apk_rope_req */
+    uint32_t n;
+    float scale;
+    int causal;
+    uint32_t window;
+    void *ws;                 /* device scratch of apk_attend_pages_ws bytes, 256-byte aligned; calls that may run at
+                               * the same time (two streams, two captured graphs) each have their own */
+    size_t ws_bytes;
+} apk_attend_req;
+/* The scratch a request needs (its pointers are not read); 0 for one that would be refused. */
+size_t apk_attend_pages_ws(apk_ctx *ctx, const apk_attend_req *req);
+/* wait != 0: synchronises the stream and reports an expired device-side wait. */
+int apk_attend_pages(apk_ctx *ctx, const apk_attend_req *req, void *stream, int wait);
 
 /* Human-readable reason for the last non-zero status on this thread
  * (gpu::init_error, stub.rs:51-53; DecodeDecline{stage,reason} gpu/types.rs:247-252). */
