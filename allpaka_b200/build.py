@@ -15,7 +15,7 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libapk_b200.so")
 SOURCES = ["apk_b200.cu", "mv_q8_0.cu", "mv_q5_0.cu", "mv_q2_k.cu", "mv_q4_k.cu", "mv_q5_k.cu", "mv_q6_k.cu",
            "pages.cu", "pages_attn.cu"]
-DEPS = SOURCES + ["decode.inl", "noalloc.inl", "gguf.inl", "kernels.cuh", "mv_pick.h", "pages.inl", "pages.cuh",
+DEPS = SOURCES + ["decode.inl", "noalloc.inl", "gguf.inl", "kernels.cuh", "mv_pick.h", "pages.inl", "pages.cuh", "pages_tc.cuh",
                   os.path.join("..", "..", "include", "allpaka_b200.h")]
 
 NVCC_FLAGS = [

@@ -9,11 +9,14 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace apk {
 
 enum { PTY_F32 = 0, PTY_F16 = 1, PTY_BF16 = 30 };  // GGML type ids
 
-constexpr int PAGES_MAX_LIST = 1024;  // sequences that one reserve, fork or release names
+constexpr int PAGES_MAX_LIST = 1024;   // sequences that one reserve, fork or release names
+constexpr int PAGES_MAX_BATCH = 4096;  // sequences of one batch of rows
 
 // work[]: what the kernels of one pool hand on to one another
 constexpr int PW_SHORT = 0;    // reserve: pages that were missing (0: done, -1: a row of the table is too short)
@@ -38,14 +41,14 @@ struct BatchDev {
 
 struct SeqRows { int slot, first, rows, len; };
 
-__device__ __forceinline__ int pages_len(const PagesDev &P, int slot) {
+__host__ __device__ __forceinline__ int pages_len(const PagesDev &P, int slot) {
     const long long cap = (long long)P.width << P.shift;
     const int len = P.lens[slot];
     return len < 0 ? 0 : ((long long)len > cap ? (int)cap : len);
 }
 
 // Sequence i of the batch, with everything clamped to what exists; a slot outside the table has no positions.
-__device__ __forceinline__ SeqRows batch_seq(const PagesDev &P, const BatchDev &B, int i) {
+__host__ __device__ __forceinline__ SeqRows batch_seq(const PagesDev &P, const BatchDev &B, int i) {
     SeqRows s;
     const int a = min(max(B.cu[i], 0), B.rows), b = min(max(B.cu[i + 1], a), B.rows);
     s.first = a;
@@ -61,7 +64,7 @@ __device__ __forceinline__ SeqRows batch_seq(const PagesDev &P, const BatchDev &
 }
 
 // The sequence that row t belongs to; -1: none.
-__device__ __forceinline__ int batch_find(const BatchDev &B, int t) {
+__host__ __device__ __forceinline__ int batch_find(const BatchDev &B, int t) {
     int lo = 0, hi = B.n;  // the last i with cu[i] <= t
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
@@ -73,7 +76,7 @@ __device__ __forceinline__ int batch_find(const BatchDev &B, int t) {
 }
 
 // Page that holds position j of a slot; -1: none.
-__device__ __forceinline__ int page_of(const PagesDev &P, int slot, int j) {
+__host__ __device__ __forceinline__ int page_of(const PagesDev &P, int slot, int j) {
     const int p = P.table[(long long)slot * P.table_stride + (j >> P.shift)];
     return (unsigned)p < (unsigned)P.n_pages ? p : -1;
 }
@@ -114,7 +117,8 @@ struct SlotList {
 };
 
 cudaError_t launch_rope_append(const RopeParams &p, int n_sm, cudaStream_t st, int *launches);
-cudaError_t launch_attend(const AttendParams &p, int n_sm, cudaStream_t st, int *launches);
+size_t attend_ws_bytes(const AttendParams &p, int n_sm);
+cudaError_t launch_attend(const AttendParams &p, int n_sm, void *ws, long long wait_limit, cudaStream_t st, int *launches);
 cudaError_t launch_pages_fork(const PagesDev &P, const SlotList &l, cudaStream_t st, int *launches);
 cudaError_t launch_pages_release(const PagesDev &P, const SlotList &l, cudaStream_t st, int *launches);
 cudaError_t launch_pages_reserve(const PagesDev &P, const SlotList &l, int n_sm, cudaStream_t st, int *launches);

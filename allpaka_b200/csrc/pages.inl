@@ -5,7 +5,7 @@
 #include <cmath>
 
 static_assert(APK_TY_F32 == PTY_F32 && APK_TY_F16 == PTY_F16 && APK_TY_BF16 == PTY_BF16, "type ids");
-static_assert(APK_PAGES_MAX_LIST == PAGES_MAX_LIST, "list length");
+static_assert(APK_PAGES_MAX_LIST == PAGES_MAX_LIST && APK_PAGES_MAX_BATCH == PAGES_MAX_BATCH, "list lengths");
 
 namespace {
 
@@ -223,12 +223,13 @@ int apk_rope_append(apk_ctx *c, const apk_rope_req *r, void *stream, int wait) {
     return wait ? pages_wait(what, p.P, (cudaStream_t)stream, false) : APK_OK;
 }
 
-size_t apk_attend_pages_ws(apk_ctx *, const apk_attend_req *) { return 0; }
+}  // extern "C"
 
-int apk_attend_pages(apk_ctx *c, const apk_attend_req *r, void *stream, int wait) {
+namespace {
+
+int attend_view(const apk_attend_req *r, AttendParams *q) {
     const char *what = "attend_pages";
-    if (!c || !r) return fail(APK_ERR_INVALID_ARG, "%s: null argument", what);
-    AttendParams p{};
+    AttendParams &p = *q;
     APK_TRY(pages_view(what, r->pages, &p.P));
     APK_TRY(pages_batch(what, r->cu, r->seqs, r->n, r->n_rows, &p.B));
     if (!r->q || !r->out) return fail(APK_ERR_INVALID_ARG, "%s: null rows", what);
@@ -254,11 +255,37 @@ int apk_attend_pages(apk_ctx *c, const apk_attend_req *r, void *stream, int wait
     p.scale_log2 = r->scale * 1.44269504088896340736f;
     p.causal = r->causal != 0;
     p.window = (int)r->window;
+    // the kernels count (kv head, tile of rows, 128 positions) in 32 bits
+    const uint64_t tiles = (uint64_t)r->n_rows / (2u * (128u / (uint32_t)p.group)) + r->n;
+    if (tiles * ((uint64_t)r->pages->width * r->pages->page / 128 + 3) * kv >= (1ull << 30))
+        return fail(APK_DECLINE_UNSUPPORTED_SHAPE, "%s: %u rows of %u sequences over tables of %u pages are too much for one call", what, r->n_rows, r->n, r->pages->width);
+    return APK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t apk_attend_pages_ws(apk_ctx *c, const apk_attend_req *r) {
+    AttendParams p{};
+    if (!c || !r || attend_view(r, &p) != APK_OK) return 0;
+    return attend_ws_bytes(p, c->n_sm);
+}
+
+int apk_attend_pages(apk_ctx *c, const apk_attend_req *r, void *stream, int wait) {
+    const char *what = "attend_pages";
+    if (!c || !r) return fail(APK_ERR_INVALID_ARG, "%s: null argument", what);
+    AttendParams p{};
+    APK_TRY(attend_view(r, &p));
     if (r->n == 0 || r->n_rows == 0) return APK_OK;
+    const size_t need = attend_ws_bytes(p, c->n_sm);
+    if (need && (!r->ws || r->ws_bytes < need || ((uintptr_t)r->ws & 255)))
+        return fail(APK_ERR_INVALID_ARG, "%s: a workspace of %zu bytes (%zu are needed, 256-byte aligned)", what, r->ws ? r->ws_bytes : (size_t)0, need);
     DeviceScope dev;
     CUDA_TRY(dev.enter(c->device));
     int launches = 0;
-    const cudaError_t e = launch_attend(p, c->n_sm, (cudaStream_t)stream, &launches);
+    const cudaError_t e = launch_attend(p, c->n_sm, r->ws, c->wait_limit, (cudaStream_t)stream, &launches);
+    if (e == cudaErrorNotSupported) return fail(APK_DECLINE_UNSUPPORTED_SHAPE, "%s: strides of the pages that a tensor map cannot express", what);
     APK_TRY(pages_done(c, e, launches, what));
     return wait ? pages_wait(what, p.P, (cudaStream_t)stream, false) : APK_OK;
 }
