@@ -1,7 +1,5 @@
 // Attention of new rows over a paged KV cache.
 //
-// Two kernels.  16-bit rows run on the tensor cores (attend_tc_kernel); 32-bit rows, which those cannot carry at their
-// precision, on the CUDA cores (attend_rows_kernel).
 #include "pages.cuh"
 #include "pages_tc.cuh"
 
@@ -80,19 +78,7 @@ __device__ __noinline__ void attend_row(const AttendParams &p, const SeqRows &s,
     for (int e = 0; e < E; ++e) from_f32(out + e, o[e] * inv);
 }
 
-template <int D, int TY, bool BF>
-__global__ void __launch_bounds__(256) attend_rows_kernel(const __grid_constant__ AttendParams p) {
-    typedef typename Elem<TY>::T T;
-    typedef typename Elem<BF ? PTY_BF16 : PTY_F16>::T C;
-    const long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int t = (int)(u / p.heads), h = (int)(u % p.heads);
-    if (t >= p.B.rows) return;
-    const int i = batch_find(p.B, t);
-    if (i < 0) return;
-    attend_row<D, T, C>(p, batch_seq(p.P, p.B, i), t, h, threadIdx.x & 31);
-}
-
-// ------------------------------------------------------------------------------------ 16-bit rows: tensor cores
+// ----------------------------------------------------------------------------------------------- tensor cores
 //
 // A tile is one kv head and up to 256 query rows of one sequence (tokens x heads of the GQA group), its work the
 // 128-position blocks of K and V that its rows see.  One CTA per SM; the blocks of all tiles in a row are cut into equal
@@ -109,6 +95,11 @@ __global__ void __launch_bounds__(256) attend_rows_kernel(const __grid_constant_
 //   and group 0 joins the two results, which lie on the same TMEM lanes.
 // The maximum that the weights refer to moves only when a row's grows by more than 2^8 (LAZY): until then weights are at
 // most 2^8 (x 2^7 for f16, whose range is 2^-24 .. 2^16), and O keeps its scale.
+//
+// 32-bit rows (over f16 pages): a query, scaled by a power of two of its own, and a weight are each the sum of two f16
+// values, 22 bits; every product is done for both.  The tensor cores' sums are truncated at about 24 bits, and over the
+// blocks of a long sequence that would add up to 2^-15: so O of a block starts from 0, and group 1 adds it to its registers
+// in 32 bits, while group 0 does the softmax of every block (tiles are narrow, two score and two O buffers).
 
 constexpr int TC_THREADS = 384;      // warps 0-7 softmax, 8 copies, 9 tensor instructions, 10 and 11 only complete the third register group
 constexpr int TC_STAGES = 4;
@@ -130,7 +121,7 @@ struct TcParams {
 struct TcGeom { int tq, step; };  // tokens per 128 rows, per tile
 __host__ __device__ __forceinline__ TcGeom tc_geom(const AttendParams &p) {
     const int tq = 128 / p.group;
-    return {tq, 2 * tq};
+    return {tq, p.ty == PTY_F32 ? tq : 2 * tq};
 }
 
 struct TcTile {
@@ -241,11 +232,13 @@ struct TcWalk {
 };
 
 struct TcShared {
-    uint64_t full[TC_STAGES], empty[TC_STAGES], q_full, s_full[2], p_full[2], o_full[2], drain;
+    uint64_t full[TC_STAGES], empty[TC_STAGES], q_full, s_full[2], p_full[2], o_full[2], o_free[2], drain;
     uint32_t tmem;
     int dead, odd;          // a wait ran out; a result is not finite
     int begin[8], end[8];   // the CTA's range: sequence, tile, head, block, and the tile's first unit
-    float ml[128][2];       // narrow tiles: maxima and sums of group 1
+    float ml[128][2];       // narrow tiles: maxima and sums of the other group
+    float by[2][128];       // 32-bit rows: what a block's new maximum makes of the sums so far
+    float unit[128];        // 32-bit rows: a row's power of two
     TcWalk walk[10];
     int prefix[1];          // [n + 1] units before each sequence
 };
@@ -275,6 +268,7 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {  // a in the low 
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
 }
+__device__ __forceinline__ float2 unpack16(uint32_t x) { return __half22float2(*(const __half2 *)&x); }
 // Values that a load into registers has delivered may not be used before its wait: ties the registers to this place.
 __device__ __forceinline__ void pin32(uint32_t *r) {
 #pragma unroll
@@ -289,10 +283,12 @@ __device__ __forceinline__ bool softmax_bar_or(bool x) {  // the 256 threads of 
 
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
 
-template <int D, bool BF>
+template <int D, int TY>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     constexpr int PANELS = D / 64;
+    constexpr bool BF = TY == PTY_BF16, F32 = TY == PTY_F32;
+    constexpr int PARTS = F32 ? 2 : 1;
     constexpr uint32_t TILE = TC_BLOCK * D * 2;    // bytes of a Q tile or of a block of K or V
     constexpr uint32_t O_COL = 256;                // TMEM columns: S0 S1 O0 O1
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -306,7 +302,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
     if (tid == 0) {
         for (int i = 0; i < TC_STAGES; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
         mbar_init(&sh.q_full, 8);
-        for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 4); mbar_init(&sh.o_full[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 4); mbar_init(&sh.o_full[i], 1); mbar_init(&sh.o_free[i], 4); }
         mbar_init(&sh.drain, 1);
         sh.dead = sh.odd = 0;
         fence_mbar_init();
@@ -423,18 +419,24 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
             const uint32_t q_addr = smem_u32(qs), r_addr = smem_u32(ring);
             auto qk = [&](int w, int tile, int st) {
                 const uint32_t qa = q_addr + tile * TILE, ka = r_addr + st * TILE;
+                // (low parts first: a sum is truncated where it is, and theirs are small)
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (k >> 2) * (TC_BLOCK * 128) + (k & 3) * 32;
-                    tc_mma_ss(tmem + w * 128, tc_desc(qa + off, 16), tc_desc(ka + off, 16), idesc_qk, k > 0);
-                }
+                for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint32_t off = (k >> 2) * (TC_BLOCK * 128) + (k & 3) * 32;
+                        tc_mma_ss(tmem + w * 128, tc_desc(qa + part * TILE + off, 16), tc_desc(ka + off, 16), idesc_qk, part < PARTS - 1 || k > 0);
+                    }
                 tc_commit(&sh.s_full[w]);
             };
             auto pv = [&](int w, int st, bool add) {
                 const uint32_t va = r_addr + st * TILE;
 #pragma unroll
-                for (int k = 0; k < TC_BLOCK / 16; ++k)
-                    tc_mma_ts(tmem + O_COL + w * D, tmem + w * 128 + k * 8, tc_desc(va + k * 2048, TC_BLOCK * 128), idesc_pv, add || k > 0);
+                for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                    for (int k = 0; k < TC_BLOCK / 16; ++k)
+                        tc_mma_ts(tmem + O_COL + w * D, tmem + w * 128 + part * 64 + k * 8, tc_desc(va + k * 2048, TC_BLOCK * 128), idesc_pv,
+                                  add || part < PARTS - 1 || k > 0);
             };
             auto full = [&](int idx) { return tc_wait(sh, &sh.full[idx % TC_STAGES], (idx / TC_STAGES) & 1, p, 2); };
             auto weights = [&](int w) {
@@ -449,7 +451,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                 const bool wide = wk.x.ntok > g.tq;
                 if (!(ok = tc_wait(sh, &sh.q_full, ph_q, p, 4))) break;
                 ph_q ^= 1;
-                if (wide) {
+                if (!F32 && wide) {
                     if (!(ok = full(ring0))) break;
                     tc_fence_after();
                     qk(0, 0, ring0 % TC_STAGES);
@@ -486,14 +488,15 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                     for (int j = 0; ok && j < n; ++j) {
                         const int w = j & 1, v = ring0 + tc_slot_v(false, j, n), kn = ring0 + tc_slot_k(false, j + 2);
                         if (!(ok = full(v) && weights(w))) break;
-                        pv(w, v % TC_STAGES, j > 1);
+                        pv(w, v % TC_STAGES, !F32 && j > 1);
                         tc_commit(&sh.empty[v % TC_STAGES]);
+                        if (F32) tc_commit(&sh.o_full[w]);
                         if (j + 2 < n) {
                             if (!(ok = full(kn))) break;
                             tc_fence_after();
                             qk(w, 0, kn % TC_STAGES);
                             tc_commit(&sh.empty[kn % TC_STAGES]);
-                        } else {
+                        } else if (!F32) {
                             tc_commit(&sh.o_full[w]);
                         }
                     }
@@ -513,7 +516,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
         const bool flip = a.scale_log2 < 0.f;                // a negative scale turns the queries round
         const float c = fmaxf(fabsf(a.scale_log2), 1e-30f);  // (a scale of 0: hidden positions still get 2^-inf)
         const float shift = BF ? 0.f : 7.f;
-        uint32_t ph_s = 0, ph_o[2] = {0, 0};
+        uint32_t ph_s = 0, ph_b = 0, ph_o[2] = {0, 0};
         bool ok = true, meta = false;
         auto wait = [&](uint64_t *bar, uint32_t parity, int site) { ok = __all_sync(~0u, ok && tc_wait(sh, bar, parity, p, site)); return ok; };
         for (bool more = step(true); more; more = step(false)) {
@@ -538,6 +541,31 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                 const int n_rows = wide && w ? (x.ntok - g.tq) * a.group : rows;
                 const int nth = wide ? 128 : 256, me = wide ? r : tid;
                 uint8_t *q_tile = qs + (wide ? w * TILE : 0);
+                if constexpr (F32) {
+                    constexpr int E = D / 32;
+                    for (int rr = warp; rr < n_rows; rr += 8) {
+                        const float *src = (const float *)a.q + (long long)(x.s.first + tok_a + rr / a.group) * a.qs[0] +
+                                           (long long)(x.h * a.group + rr % a.group) * a.qs[1] + lane * E;
+                        float v[E], mx = 0.f;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) { v[e] = src[e]; mx = fmaxf(mx, fabsf(v[e])); }
+                        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+                        // the row's largest value lands in [2^13, 2^14): what is 2^-27 of it still has 11 bits
+                        const int ex = mx < INFINITY ? max((int)(__float_as_uint(mx) >> 23) - 127, -100) : 0;
+                        const float by = __uint_as_float((uint32_t)(127 + 13 - ex) << 23) * (flip ? -1.f : 1.f);
+                        if (lane == 0) sh.unit[rr] = __uint_as_float((uint32_t)max(127 - 13 + ex, 1) << 23);
+#pragma unroll
+                        for (int e = 0; e < E; e += 2) {
+                            const float u0 = v[e] * by, u1 = v[e + 1] * by;
+                            const uint32_t hi = pack16<false>(u0, u1);
+                            const float2 h = unpack16(hi);
+                            const int d = lane * E + e;
+                            uint8_t *at = q_tile + (d >> 6) * (TC_BLOCK * 128) + sw128(rr, (d >> 3) & 7) + (d & 7) * 2;
+                            *(uint32_t *)at = hi;
+                            *(uint32_t *)(at + TILE) = pack16<false>(u0 - h.x, u1 - h.y);
+                        }
+                    }
+                } else
                 for (int i = me; i < n_rows * (D / 8); i += nth) {
                     const int rr = i / (D / 8), ch = i % (D / 8);
                     const uint16_t *src = (const uint16_t *)a.q + (long long)(x.s.first + tok_a + rr / a.group) * a.qs[0] +
@@ -552,6 +580,131 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
             }
             float m = -INFINITY, l = 0.f;   // m: of the scaled scores, what the weights refer to
             const bool warp_mine = __any_sync(~0u, mine);
+            // scores of positions that the row does not see
+            auto hide = [&](float *f, int pos) {
+                                    if (odd || __any_sync(~0u, mine && (pos < lo || pos + TC_BLOCK > hi))) {
+                                        uint32_t see[4];   // a bit per position
+                #pragma unroll
+                                        for (int k = 0; k < 4; ++k) see[k] = bits_below(hi - pos - 32 * k) & ~bits_below(lo - pos - 32 * k);
+                                        if (odd)
+                                            for (int at = pos; at < min(pos + TC_BLOCK, x.s.len); at += min(a.P.page, 32))
+                                                if (page_of(a.P, x.s.slot, at) < 0) {
+                                                    const uint32_t gone = bits_below(min(a.P.page, 32)) << (at & 31);
+                #pragma unroll
+                                                    for (int k = 0; k < 4; ++k)
+                                                        if (((at - pos) >> 5) == k) see[k] &= ~gone;
+                                                }
+                #pragma unroll
+                                        for (int k = 0; k < 128; ++k)
+                                            if (!((see[k >> 5] >> (k & 31)) & 1u)) f[k] = -INFINITY;
+                                    }
+            };
+            // What lies behind the sequence in its last page takes part in the product with weight 0: it may not be NaN.
+            auto clear_tail = [&](int j, int pos) {
+                const int idx = ring0 + tc_slot_v(wide, j, n);
+                if (!wait(&sh.full[idx % TC_STAGES], (idx / TC_STAGES) & 1, 6)) return false;
+                if (pos + r >= x.s.len) {
+                    uint8_t *v = ring + (idx % TC_STAGES) * TILE + r * 128;
+#pragma unroll
+                    for (int k = 0; k < PANELS * 8; ++k) *(uint4 *)(v + (k >> 3) * (TC_BLOCK * 128) + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();
+                return true;
+            };
+            const int slot = 2 * cta + (wk.j0 == 0 ? 1 : 0);
+            if constexpr (F32) {
+                softmax_bar_or(false);   // the rows' powers of two are written
+                const float cr = c * sh.unit[r];
+                if (w == 0) {
+                    for (int j = 0; j < n && ok; ++j) {
+                        const int b = j & 1, pos = (k_first + j) * TC_BLOCK;
+                        if (!wait(&sh.s_full[b], ph_b >> b & 1, 5)) break;
+                        // (the sums of the block before last have been taken: its O buffer and its factor are free)
+                        if (!wait(&sh.o_free[b], (ph_b >> b & 1) ^ 1, 9)) break;
+                        ph_b ^= 1 << b;
+                        tc_fence_after();
+                        if (warp_mine) {
+                            const uint32_t tb = tmem + lanes + b * 128;
+                            uint32_t s[128], hi[64], lw[64];
+                            tm_ld32(tb, s); tm_ld32(tb + 32, s + 32); tm_ld32(tb + 64, s + 64); tm_ld32(tb + 96, s + 96);
+                            tm_wait_ld();
+                            pin32(s); pin32(s + 32); pin32(s + 64); pin32(s + 96);
+                            float *f = (float *)s;
+                            hide(f, pos);
+                            float mx[4] = {f[0], f[1], f[2], f[3]};
+#pragma unroll
+                            for (int k = 4; k < 128; ++k) mx[k & 3] = fmaxf(mx[k & 3], f[k]);
+                            const float to_m = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * cr);
+                            const float by = m == -INFINITY ? 0.f : ex2(m - to_m);
+                            m = to_m;
+                            sh.by[b][r] = by;
+                            const float off = m == -INFINITY ? 0.f : -m;
+                            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int k = 0; k < 128; k += 2) {
+                                // weights up to 2^14 (f16 ends at 2^16); as a factor: in the exponent it would cost the argument bits
+                                const float p0 = 16384.f * ex2(fmaf(f[k], cr, off)), p1 = 16384.f * ex2(fmaf(f[k + 1], cr, off));
+                                sum[(k >> 1) & 3] += p0 + p1;
+                                hi[k >> 1] = pack16<false>(p0, p1);
+                                const float2 h = unpack16(hi[k >> 1]);
+                                lw[k >> 1] = pack16<false>(p0 - h.x, p1 - h.y);
+                            }
+                            l = l * by + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                            tm_st32(tb, hi); tm_st32(tb + 32, hi + 32); tm_st32(tb + 64, lw); tm_st32(tb + 96, lw + 32);
+                            tm_wait_st();
+                        }
+                        if (pos + TC_BLOCK > x.s.len && !clear_tail(j, pos)) break;
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.p_full[b]);
+                    }
+                    sh.ml[r][0] = m;
+                    sh.ml[r][1] = l;
+                    softmax_bar_or(false);
+                } else {
+                    float acc[D];
+#pragma unroll
+                    for (int k = 0; k < D; ++k) acc[k] = 0.f;
+                    for (int j = 0; j < n && ok; ++j) {
+                        const int b = j & 1;
+                        if (!wait(&sh.p_full[b], ph_b >> b & 1, 7)) break;   // (the factor)
+                        if (!wait(&sh.o_full[b], ph_b >> b & 1, 8)) break;
+                        ph_b ^= 1 << b;
+                        tc_fence_after();
+                        if (warp_mine) {
+                            const float by = sh.by[b][r];
+#pragma unroll
+                            for (int h = 0; h < D; h += 32) {
+                                uint32_t o[32];
+                                tm_ld32(tmem + lanes + O_COL + b * D + h, o);
+                                tm_wait_ld();
+                                pin32(o);
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) acc[h + k] = fmaf(acc[h + k], by, __uint_as_float(o[k]));
+                            }
+                        }
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.o_free[b]);
+                    }
+                    softmax_bar_or(false);
+                    const float top = sh.ml[r][0], lt = sh.ml[r][1], inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
+                    float *dst = whole ? (float *)a.out + row * a.os[0] + head * a.os[1] : p.part + ((long long)slot * p.ws_rows + r) * D;
+                    float size = 0.f;
+                    if (mine && ok) {
+#pragma unroll
+                        for (int k = 0; k < D; k += 4) {
+                            const float u = whole ? inv : 1.f;
+                            const float4 y = make_float4(acc[k] * u, acc[k + 1] * u, acc[k + 2] * u, acc[k + 3] * u);
+                            size += (fabsf(y.x) + fabsf(y.y)) + (fabsf(y.z) + fabsf(y.w));
+                            *(float4 *)(dst + k) = y;
+                        }
+                        if (!whole) *(float2 *)(p.ml + ((long long)slot * p.ws_rows + r) * 2) = make_float2(top, lt);
+                        else if (!(size < INFINITY)) sh.odd = 1;   // (see attend_join_kernel)
+                    }
+                }
+                ring0 += 2 * n;
+            } else {
             const int cnt = wide ? n : (n - w + 1) >> 1;
             for (int i = 0; i < cnt && ok; ++i) {
                 const int j = wide ? i : 2 * i + w, pos = (k_first + j) * TC_BLOCK;
@@ -564,22 +717,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                     tm_wait_ld();
                     pin32(s); pin32(s + 32); pin32(s + 64); pin32(s + 96);
                     float *f = (float *)s;
-                    if (odd || __any_sync(~0u, pos < lo || pos + TC_BLOCK > hi)) {
-                        uint32_t see[4];   // a bit per position
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) see[k] = bits_below(hi - pos - 32 * k) & ~bits_below(lo - pos - 32 * k);
-                        if (odd)
-                            for (int at = pos; at < min(pos + TC_BLOCK, x.s.len); at += min(a.P.page, 32))
-                                if (page_of(a.P, x.s.slot, at) < 0) {
-                                    const uint32_t gone = bits_below(min(a.P.page, 32)) << (at & 31);
-#pragma unroll
-                                    for (int k = 0; k < 4; ++k)
-                                        if (((at - pos) >> 5) == k) see[k] &= ~gone;
-                                }
-#pragma unroll
-                        for (int k = 0; k < 128; ++k)
-                            if (!((see[k >> 5] >> (k & 31)) & 1u)) f[k] = -INFINITY;
-                    }
+                    hide(f, pos);
                     float mx = f[0];
 #pragma unroll
                     for (int k = 1; k < 128; ++k) mx = fmaxf(mx, f[k]);
@@ -617,17 +755,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                     tm_st32(ts + 32, s + 32);
                     tm_wait_st();
                 }
-                if (pos + TC_BLOCK > x.s.len) {
-                    // what lies behind the sequence in its last page takes part in the product with weight 0: it may not be NaN
-                    const int idx = ring0 + tc_slot_v(wide, j, n);
-                    if (!wait(&sh.full[idx % TC_STAGES], (idx / TC_STAGES) & 1, 6)) break;
-                    if (pos + r >= x.s.len) {
-                        uint8_t *v = ring + (idx % TC_STAGES) * TILE + r * 128;
-#pragma unroll
-                        for (int k = 0; k < PANELS * 8; ++k) *(uint4 *)(v + (k >> 3) * (TC_BLOCK * 128) + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_async_smem();
-                }
+                if (pos + TC_BLOCK > x.s.len && !clear_tail(j, pos)) break;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.p_full[w]);
@@ -657,7 +785,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                 const float lt = l * b0 + l1 * b1;
                 const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
                 float size = 0.f;
-                const int slot = 2 * cta + (wk.j0 == 0 ? 1 : 0), wr = wide ? w * 128 + r : r;
+                const int wr = wide ? w * 128 + r : r;
                 const bool part = mine && !whole;
                 if (warp_mine && ok) {
                     uint16_t *out = (uint16_t *)a.out + row * a.os[0] + head * a.os[1];
@@ -703,6 +831,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
             } else if (n > 1) {
                 ph_o[1] ^= 1;
             }
+            }
             // the first of a cut tile's pieces says how many follow
             if (!whole && wk.j0 == 0) {
                 meta = true;
@@ -736,10 +865,11 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
 // the others in slot 0 of the CTAs behind it.  A warp per row, in the order of the pieces.
 // An infinity or NaN in V at a position that some rows of a tile do not see has met their weight of 0 in the product.  Such
 // rows show it by not being finite; they are done over here, position by position.
-template <int D, bool BF>
+template <int D, int TY>
 __global__ void __launch_bounds__(512) attend_join_kernel(const __grid_constant__ TcParams p) {
     constexpr int E = D / 32;
-    typedef typename Elem<BF ? PTY_BF16 : PTY_F16>::T T;
+    typedef typename Elem<TY>::T T;
+    typedef typename Elem<TY == PTY_BF16 ? PTY_BF16 : PTY_F16>::T C;
     const AttendParams &a = p.a;
     const int *mt = p.meta + blockIdx.x * 8;
     const int more = mt[0];
@@ -753,7 +883,7 @@ __global__ void __launch_bounds__(512) attend_join_kernel(const __grid_constant_
             const T *o = (const T *)a.out + t * a.os[0] + hd * a.os[1] + (threadIdx.x & 31) * E;
             float size = 0.f;
             for (int e = 0; e < E; ++e) size += fabsf(to_f32(o[e]));
-            if (__any_sync(~0u, !(size < INFINITY))) attend_row<D, T, T>(a, batch_seq(a.P, a.B, i), t, hd, threadIdx.x & 31);
+            if (__any_sync(~0u, !(size < INFINITY))) attend_row<D, T, C>(a, batch_seq(a.P, a.B, i), t, hd, threadIdx.x & 31);
         }
     }
     if (more <= 0 || more >= p.n_ctas - (int)blockIdx.x) return;
@@ -781,11 +911,11 @@ __global__ void __launch_bounds__(512) attend_join_kernel(const __grid_constant_
         float size = 0.f;
         for (int e = 0; e < E; ++e) { o[e] *= inv; size += fabsf(o[e]); }
         const int row = s.first + tok0 + tok, head = h * a.group + rr % a.group;
-        uint16_t *out = (uint16_t *)a.out + row * a.os[0] + head * a.os[1] + lane * E;
-        for (int e = 0; e < E; e += 2) *(uint32_t *)(out + e) = pack16<BF>(o[e], o[e + 1]);
+        T *out = (T *)a.out + row * a.os[0] + head * a.os[1] + lane * E;
+        for (int e = 0; e < E; ++e) from_f32(out + e, o[e]);
         if (__any_sync(~0u, !(size < INFINITY))) {
             __syncwarp();
-            attend_row<D, T, T>(a, s, row, head, lane);
+            attend_row<D, T, C>(a, s, row, head, lane);
         }
     }
 }
@@ -820,15 +950,15 @@ bool page_map(CUtensorMap *m, const PagesDev &P, const uint16_t *base, const lon
 struct TcSize { size_t meta, ml, part; int rows; };
 TcSize tc_size(const AttendParams &p, int n_sm) {
     TcSize s;
-    const int tq = 128 / p.group;
-    s.rows = p.B.rows > tq ? 256 : p.B.rows * p.group;
+    const TcGeom g = tc_geom(p);
+    s.rows = p.B.rows > g.tq ? (g.step > g.tq ? 256 : 128) : p.B.rows * p.group;
     s.meta = ((size_t)n_sm * 8 * 4 + 255) / 256 * 256;
     s.ml = ((size_t)n_sm * 2 * s.rows * 2 * 4 + 255) / 256 * 256;
     s.part = (size_t)n_sm * 2 * s.rows * p.P.dim * 4;
     return s;
 }
 
-template <int D, bool BF>
+template <int D, int TY>
 cudaError_t launch_tc(const AttendParams &p, int n_sm, void *ws, long long wait_limit, cudaStream_t st, int *launches) {
     constexpr int smem = 1024 + (2 + TC_STAGES) * TC_BLOCK * D * 2 + (int)sizeof(TcShared) + 4 * PAGES_MAX_BATCH;
     static_assert(smem <= 232448, "shared memory of a block");
@@ -844,39 +974,28 @@ cudaError_t launch_tc(const AttendParams &p, int n_sm, void *ws, long long wait_
     q.part = (float *)((char *)ws + z.meta + z.ml);
     q.wait_limit = wait_limit;
     // (the limit belongs to the kernel on the current device; setting it again costs a few hundred nanoseconds)
-    cudaError_t e = cudaFuncSetAttribute(attend_tc_kernel<D, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(attend_tc_kernel<D, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    attend_tc_kernel<D, BF><<<n_sm, TC_THREADS, smem, st>>>(q, km, vm);
+    attend_tc_kernel<D, TY><<<n_sm, TC_THREADS, smem, st>>>(q, km, vm);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    attend_join_kernel<D, BF><<<dim3(n_sm, z.rows == 256 ? 4 : 1), 512, 0, st>>>(q);
+    attend_join_kernel<D, TY><<<dim3(n_sm, z.rows == 256 ? 4 : 1), 512, 0, st>>>(q);
     *launches += 2;
-    return cudaGetLastError();
-}
-
-template <int D>
-cudaError_t launch_rows(const AttendParams &p, cudaStream_t st, int *launches) {
-    const unsigned grid = (unsigned)(((long long)p.B.rows * p.heads + 7) / 8);
-    if (p.ty == PTY_F32) attend_rows_kernel<D, PTY_F32, false><<<grid, 256, 0, st>>>(p);
-    else if (p.ty == PTY_F16) attend_rows_kernel<D, PTY_F16, false><<<grid, 256, 0, st>>>(p);
-    else attend_rows_kernel<D, PTY_BF16, true><<<grid, 256, 0, st>>>(p);
-    *launches += 1;
     return cudaGetLastError();
 }
 
 }  // namespace
 
 size_t attend_ws_bytes(const AttendParams &p, int n_sm) {
-    if (p.ty == PTY_F32) return 0;
     const TcSize z = tc_size(p, n_sm);
     return z.meta + z.ml + z.part;
 }
 
 cudaError_t launch_attend(const AttendParams &p, int n_sm, void *ws, long long wait_limit, cudaStream_t st, int *launches) {
-    if (p.ty == PTY_F32) return p.P.dim == 128 ? launch_rows<128>(p, st, launches) : launch_rows<64>(p, st, launches);
-    if (p.P.dim == 128)
-        return p.P.bf16 ? launch_tc<128, true>(p, n_sm, ws, wait_limit, st, launches) : launch_tc<128, false>(p, n_sm, ws, wait_limit, st, launches);
-    return p.P.bf16 ? launch_tc<64, true>(p, n_sm, ws, wait_limit, st, launches) : launch_tc<64, false>(p, n_sm, ws, wait_limit, st, launches);
+    const bool d128 = p.P.dim == 128;
+    if (p.ty == PTY_F32) return (d128 ? launch_tc<128, PTY_F32> : launch_tc<64, PTY_F32>)(p, n_sm, ws, wait_limit, st, launches);
+    if (p.ty == PTY_BF16) return (d128 ? launch_tc<128, PTY_BF16> : launch_tc<64, PTY_BF16>)(p, n_sm, ws, wait_limit, st, launches);
+    return (d128 ? launch_tc<128, PTY_F16> : launch_tc<64, PTY_F16>)(p, n_sm, ws, wait_limit, st, launches);
 }
 
 }  // namespace apk
