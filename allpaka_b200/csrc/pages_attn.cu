@@ -8,6 +8,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <climits>
 
 namespace apk {
 namespace {
@@ -86,13 +87,14 @@ __device__ __noinline__ void attend_row(const AttendParams &p, const SeqRows &s,
 // a cut runs through leaves partial results (unnormalised rows, maximum, sum) in the workspace, which
 // attend_join_kernel merges in a fixed order.
 //
-// Ten warps: two groups of four for the softmax (thread = row = TMEM lane), one that issues TMA copies, one that issues
-// the tensor instructions.  S = Q K^T (both from shared memory) goes to TMEM; the softmax group turns its 128 x 128
+// Two groups of four warps for the softmax (thread = row = TMEM lane), a warp that walks the CTA's range and hands out its
+// segments, one that issues TMA copies, one that issues the tensor instructions.  S = Q K^T (both from shared memory) goes to TMEM; the softmax group turns its 128 x 128
 // scores into 16-bit weights P over the same TMEM columns; O += P V takes P from TMEM and V from shared memory
 // (transposed by its descriptor).
 //   wide tile (more than 128 rows): group w works on rows 128w.. and shares every K and V block with the other;
 //   narrow tile (one token of a few heads, mostly): both groups hold the same rows, group w takes every second block,
-//   and group 0 joins the two results, which lie on the same TMEM lanes.
+//   and group 0 joins the two results, which lie on the same TMEM lanes.  Up to 32 rows lie in TMEM four times, and each
+//   copy weighs a quarter of a block's positions: one warp would otherwise do it all.
 // The maximum that the weights refer to moves only when a row's grows by more than 2^8 (LAZY): until then weights are at
 // most 2^8 (x 2^7 for f16, whose range is 2^-24 .. 2^16), and O keeps its scale.
 //
@@ -101,12 +103,14 @@ __device__ __noinline__ void attend_row(const AttendParams &p, const SeqRows &s,
 // blocks of a long sequence that would add up to 2^-15: so O of a block starts from 0, and group 1 adds it to its registers
 // in 32 bits, while group 0 does the softmax of every block (tiles are narrow, two score and two O buffers).
 
-constexpr int TC_THREADS = 384;      // warps 0-7 softmax, 8 copies, 9 tensor instructions, 10 and 11 only complete the third register group
+constexpr int TC_THREADS = 384;      // warps 0-7 softmax, 8 copies, 9 tensor instructions, 10 walks the segments, 11 completes the third register group
 constexpr int TC_STAGES = 4;
 constexpr int TC_BLOCK = 128;         // positions a block
 constexpr int TC_OVERHEAD = 2;        // what opening and closing a tile costs, in blocks
 constexpr int TC_MIN_UNITS = 4;       // least range of a CTA
 constexpr int TC_MOST = 1 << 30;      // units of a call (the host has bounded a proper batch's)
+constexpr int TC_SEGS = 4;            // segments that are known ahead
+constexpr int TC_INFO = 256;          // sequences that a block keeps a copy of
 constexpr float TC_LAZY = 8.f;
 
 struct TcParams {
@@ -118,11 +122,15 @@ struct TcParams {
     long long wait_limit;
 };
 
-struct TcGeom { int tq, step; };  // tokens per 128 rows, per tile
-__host__ __device__ __forceinline__ TcGeom tc_geom(const AttendParams &p) {
-    const int tq = 128 / p.group;
-    return {tq, p.ty == PTY_F32 ? tq : 2 * tq};
-}
+// Everything that says how a call's work is cut.
+struct TcBatch {
+    const AttendParams &p;
+    int tq, step;           // tokens per 128 rows, per tile
+    const SeqRows *info;    // the first TC_INFO sequences, where a copy is at hand
+    __host__ __device__ __forceinline__ TcBatch(const AttendParams &p_, const SeqRows *i)
+        : p(p_), tq(128 / p_.group), step(p_.ty == PTY_F32 ? 128 / p_.group : 2 * (128 / p_.group)), info(i) {}
+    __host__ __device__ __forceinline__ SeqRows seq(int i) const { return info && i < TC_INFO ? info[i] : batch_seq(p.P, p.B, i); }
+};
 
 struct TcTile {
     int seq, t, h;          // batch index, tile of the sequence, kv head
@@ -132,51 +140,51 @@ struct TcTile {
     int tok0, ntok, k0, nb; // first token (of the sequence), tokens, first block, blocks
 };
 
-__host__ __device__ __forceinline__ void tc_span(const AttendParams &p, const TcGeom &g, TcTile &x) {
-    x.tok0 = x.t * g.step;
-    x.ntok = min(x.s.rows - x.tok0, g.step);
+__host__ __device__ __forceinline__ void tc_span(const TcBatch &c, TcTile &x) {
+    x.tok0 = x.t * c.step;
+    x.ntok = min(x.s.rows - x.tok0, c.step);
     const int pos = x.s.len - x.s.rows + x.tok0;
     int lo, hi, unused;
-    row_span(p, x.s.len, pos, lo, unused);
-    row_span(p, x.s.len, pos + x.ntok - 1, unused, hi);
+    row_span(c.p, x.s.len, pos, lo, unused);
+    row_span(c.p, x.s.len, pos + x.ntok - 1, unused, hi);
     x.k0 = lo / TC_BLOCK;
     x.nb = hi > lo ? (hi + TC_BLOCK - 1) / TC_BLOCK - x.k0 : 0;
 }
 
-__host__ __device__ __forceinline__ void tc_open(const AttendParams &p, const TcGeom &g, TcTile &x) {
-    while (x.seq < p.B.n) {
-        x.s = batch_seq(p.P, p.B, x.seq);
-        x.nt = (x.s.rows + g.step - 1) / g.step;
+__host__ __device__ __forceinline__ void tc_open(const TcBatch &c, TcTile &x) {
+    while (x.seq < c.p.B.n) {
+        x.s = c.seq(x.seq);
+        x.nt = (x.s.rows + c.step - 1) / c.step;
         if (x.nt > 0) break;
         x.seq++;
     }
-    if (x.seq < p.B.n) tc_span(p, g, x);
+    if (x.seq < c.p.B.n) tc_span(c, x);
 }
 
-__host__ __device__ __forceinline__ void tc_next(const AttendParams &p, const TcGeom &g, TcTile &x) {
+__host__ __device__ __forceinline__ void tc_next(const TcBatch &c, TcTile &x) {
     x.base += x.nb + TC_OVERHEAD;
-    if (++x.h < p.P.kv) return;
+    if (++x.h < c.p.P.kv) return;
     x.h = 0;
     if (++x.t < x.nt) {
-        tc_span(p, g, x);
+        tc_span(c, x);
         return;
     }
     x.t = 0;
     x.seq++;
-    tc_open(p, g, x);
+    tc_open(c, x);
 }
 
 // Where the cut before unit u falls: a tile and a block.  A cut that would leave a single block on one side moves to
 // the tile's edge.
-__host__ __device__ inline void tc_cut(const AttendParams &p, const TcGeom &g, const int *prefix, int total, int u, int *out) {
+__host__ __device__ inline void tc_cut(const TcBatch &c, const int *prefix, int total, int u, int *out) {
     TcTile x;
     x.t = x.h = 0;
     int block = 0;
     if (u >= total) {
-        x.seq = p.B.n;
+        x.seq = c.p.B.n;
         x.base = total;
     } else {
-        int lo = 0, hi = p.B.n;  // the last sequence with prefix <= u; it has units, since its successor's prefix is larger
+        int lo = 0, hi = c.p.B.n;  // the last sequence with prefix <= u; it has units, since its successor's prefix is larger
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (prefix[mid] <= u) lo = mid;
@@ -184,11 +192,11 @@ __host__ __device__ inline void tc_cut(const AttendParams &p, const TcGeom &g, c
         }
         x.seq = lo;
         x.base = prefix[lo];
-        tc_open(p, g, x);
-        while ((long long)x.base + (long long)(x.nb + TC_OVERHEAD) * p.P.kv <= u) {
-            x.base += (x.nb + TC_OVERHEAD) * p.P.kv;
+        tc_open(c, x);
+        while ((long long)x.base + (long long)(x.nb + TC_OVERHEAD) * c.p.P.kv <= u) {
+            x.base += (x.nb + TC_OVERHEAD) * c.p.P.kv;
             ++x.t;
-            tc_span(p, g, x);
+            tc_span(c, x);
         }
         x.h = (u - x.base) / (x.nb + TC_OVERHEAD);
         x.base += x.h * (x.nb + TC_OVERHEAD);
@@ -196,20 +204,19 @@ __host__ __device__ inline void tc_cut(const AttendParams &p, const TcGeom &g, c
         if (u == x.base || block <= 1) {
             block = 0;
         } else if (block >= x.nb - 1) {
-            tc_next(p, g, x);
+            tc_next(c, x);
             block = 0;
         }
     }
     out[0] = x.seq; out[1] = x.t; out[2] = x.h; out[3] = block; out[4] = x.base;
 }
 
-// The segments of a CTA's range, in order.  Every warp walks them for itself, in shared memory (the registers belong to
-// the scores): its first lane takes the step.
+// The segments of a CTA's range, in order.
 struct TcWalk {
     TcTile x;
     int j0, j1;   // blocks of the tile
-    __host__ __device__ __forceinline__ bool check(const AttendParams &p, const int *end) {
-        if (x.seq >= p.B.n) return false;
+    __host__ __device__ __forceinline__ bool check(const TcBatch &c, const int *end) {
+        if (x.seq >= c.p.B.n) return false;
         if (x.seq == end[0] && x.t == end[1] && x.h == end[2]) {
             j1 = end[3];
             return j1 > j0;
@@ -217,29 +224,40 @@ struct TcWalk {
         j1 = x.nb;
         return x.seq < end[0] || (x.seq == end[0] && (x.t < end[1] || (x.t == end[1] && x.h < end[2])));
     }
-    __host__ __device__ __forceinline__ bool start(const AttendParams &p, const TcGeom &g, const int *begin, const int *end) {
+    __host__ __device__ __forceinline__ bool start(const TcBatch &c, const int *begin, const int *end) {
         x.seq = begin[0]; x.t = begin[1]; x.h = begin[2]; x.base = begin[4];
         j0 = begin[3];
-        tc_open(p, g, x);
-        return check(p, end);
+        tc_open(c, x);
+        return check(c, end);
     }
-    __host__ __device__ __forceinline__ bool next(const AttendParams &p, const TcGeom &g, const int *end) {
+    __host__ __device__ __forceinline__ bool next(const TcBatch &c, const int *end) {
         if (x.seq == end[0] && x.t == end[1] && x.h == end[2]) return false;
-        tc_next(p, g, x);
+        tc_next(c, x);
         j0 = 0;
-        return check(p, end);
+        return check(c, end);
     }
 };
 
+// One segment, as the walking warp hands it to the others.
+struct TcSegment {
+    SeqRows s;
+    int h, tok0, ntok;      // kv head, first token of the sequence, tokens
+    int first, n;           // first block of the sequence, blocks; n < 0: there are no more segments
+    int base, nb, j0;       // the tile's first unit and blocks; the segment's first block of the tile
+};
+
 struct TcShared {
-    uint64_t full[TC_STAGES], empty[TC_STAGES], q_full, s_full[2], p_full[2], o_full[2], o_free[2], drain;
+    uint64_t full[TC_STAGES], empty[TC_STAGES], seg_full[TC_SEGS], seg_empty[TC_SEGS], q_full, s_full[2], p_full[2], o_full[2], o_free[2], both, half, drain;
     uint32_t tmem;
     int dead, odd;          // a wait ran out; a result is not finite
-    int begin[8], end[8];   // the CTA's range: sequence, tile, head, block, and the tile's first unit
-    float ml[128][2];       // narrow tiles: maxima and sums of the other group
+    int cut[2][8];          // where the CTA's range begins and ends: sequence, tile, head, block, and the tile's first unit
+    int gone[2][8];         // per warp: a page of the segment is not there
+    float ml[128][2];       // maxima and sums that one softmax group hands to the other
+    float red[128][2];      // ... and the lanes of one group to one another
     float by[2][128];       // 32-bit rows: what a block's new maximum makes of the sums so far
     float unit[128];        // 32-bit rows: a row's power of two
-    TcWalk walk[10];
+    TcSegment seg[TC_SEGS];
+    SeqRows info[TC_INFO];
     int prefix[1];          // [n + 1] units before each sequence
 };
 
@@ -247,13 +265,16 @@ struct TcShared {
 __host__ __device__ __forceinline__ int tc_slot_k(bool wide, int j) { return wide ? 2 * j : (j < 2 ? j : 2 * j - 1); }
 __host__ __device__ __forceinline__ int tc_slot_v(bool wide, int j, int n) { return wide ? 2 * j + 1 : (j < n - 1 ? 2 * j + 2 : 2 * n - 1); }
 
-__device__ __forceinline__ bool tc_wait(TcShared &sh, uint64_t *bar, uint32_t parity, const TcParams &p, int site) {
-    if (mbar_try_wait(bar, parity)) return true;
+// (out of line, like all that a block of scores does not need: the code of a block's loop and its registers are what counts)
+__device__ __forceinline__ bool tc_wait_on(TcShared &sh, uint64_t *bar, uint32_t parity, int *err, long long limit, int site) {
     if (*(volatile int *)&sh.dead) return false;
-    if (mbar_wait_bounded(bar, parity, p.wait_limit)) return true;
+    if (mbar_wait_bounded(bar, parity, limit)) return true;
     *(volatile int *)&sh.dead = 1;
-    atomicCAS(&p.a.P.work[PW_ERR], 0, site);
+    atomicCAS(err, 0, site);
     return false;
+}
+__device__ __forceinline__ bool tc_wait(TcShared &sh, uint64_t *bar, uint32_t parity, const TcParams &p, int site) {
+    return mbar_try_wait(bar, parity) || tc_wait_on(sh, bar, parity, &p.a.P.work[PW_ERR], p.wait_limit, site);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -274,14 +295,202 @@ __device__ __forceinline__ void pin32(uint32_t *r) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i])::"memory");
 }
-__device__ __forceinline__ bool softmax_bar_or(bool x) {  // the 256 threads of both groups
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(r) : "r"((uint32_t)x) : "memory");
-    return r != 0;
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
+
+__device__ __forceinline__ void tm_ld(uint32_t addr, uint32_t *r) {
+    tm_ld32(addr, r);
+    tm_wait_ld();
+    pin32(r);
 }
 
-__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
+// What a softmax thread knows of its row in a segment.
+struct TcRow {
+    int lo, hi;        // positions that it sees
+    bool mine, odd;    // the thread has a row; the segment has pages that are not there
+};
+
+// Scores of 32 positions from `pos` on (a multiple of 32) that the row does not see.
+__device__ __forceinline__ void tc_hide(const AttendParams &a, const SeqRows &s, const TcRow &row, int pos, float *f) {
+    uint32_t see = bits_below(row.hi - pos) & ~bits_below(row.lo - pos);   // a bit per position
+    if (row.odd)
+        for (int at = pos; at < min(pos + 32, s.len); at += min(a.P.page, 32))
+            if (page_of(a.P, s.slot, at) < 0) see &= ~(bits_below(min(a.P.page, 32)) << (at & 31));
+#pragma unroll
+    for (int k = 0; k < 32; ++k)
+        if (!((see >> k) & 1u)) f[k] = -INFINITY;
+}
+
+__device__ __forceinline__ float tc_max(const float *f) {
+    float mx[4] = {f[0], f[1], f[2], f[3]};
+#pragma unroll
+    for (int k = 4; k < 32; ++k) mx[k & 3] = fmaxf(mx[k & 3], f[k]);
+    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+
+// 32 scores into 16 columns of weights (and as many of their second parts); returns the weights' sum.
+template <bool BF>
+__device__ __forceinline__ float tc_exp16(const float *f, float c, float off, uint32_t *w) {
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 32; k += 2) {
+        const float p0 = ex2(fmaf(f[k], c, off)), p1 = ex2(fmaf(f[k + 1], c, off));
+        sum[(k >> 1) & 3] += p0 + p1;
+        w[k >> 1] = pack16<BF>(p0, p1);
+    }
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+__device__ __forceinline__ float tc_exp32(const float *f, float c, float off, uint32_t *hi, uint32_t *lw) {
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 32; k += 2) {
+        // weights up to 2^14 (f16 ends at 2^16); as a factor: in the exponent it would cost the argument bits
+        const float p0 = 16384.f * ex2(fmaf(f[k], c, off)), p1 = 16384.f * ex2(fmaf(f[k + 1], c, off));
+        sum[(k >> 1) & 3] += p0 + p1;
+        hi[k >> 1] = pack16<false>(p0, p1);
+        const float2 h = unpack16(hi[k >> 1]);
+        lw[k >> 1] = pack16<false>(p0 - h.x, p1 - h.y);
+    }
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+// A warp's quarter of the weight columns; the other quarters, whose positions other lanes weigh, get 0.
+__device__ __forceinline__ void tc_put_quarter(uint32_t to, int part, const uint32_t *w) {
+    uint32_t none[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) none[i] = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (q == part) tm_st16(to + q * 16, w);
+        else tm_st16(to + q * 16, none);
+    }
+}
+
+// What a group's sums O at `to` become where the maximum of a row has moved.
+template <int D>
+__device__ __forceinline__ void tc_rescale(uint32_t to, float by) {
+#pragma unroll 1
+    for (int h = 0; h < D; h += 32) {
+        uint32_t o[32];
+        tm_ld(to + h, o);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
+        tm_st32(to + h, o);
+    }
+}
+
+// A block of scores (TMEM columns at `ts`) becomes 16-bit weights in the same columns: chunk by chunk of 32, twice over (the
+// maximum first), since 128 scores in registers would leave too few for anything else.  The weights of a chunk lie where scores
+// have been read already.  m: what the weights refer to, l: their sum; `first`: there are no sums O yet.
+// A quarter (part >= 0): the thread weighs 32 of the positions.
+template <int D, bool BF>
+__device__ __forceinline__ void tc_weights16(const AttendParams &a, const SeqRows &s, const TcRow &row, uint32_t ts, uint32_t to, int part, int pos, bool first,
+                                             float c, float &m, float &l) {
+    uint32_t xa[32], xb[32], w[16];
+    float *const fa = (float *)xa, *const fb = (float *)xb;
+    const int p0 = part < 0 ? pos : pos + part * 32;
+    const bool edge = row.odd || __any_sync(~0u, row.mine && (p0 < row.lo || p0 + (part < 0 ? 128 : 32) > row.hi));
+    float mx;
+    if (part >= 0) {
+        tm_ld(ts + part * 32, xa);
+        if (edge) tc_hide(a, s, row, p0, fa);
+        mx = tc_max(fa);
+    } else {
+        mx = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 128; h += 64) {
+            tm_ld32(ts + h, xa);
+            tm_ld32(ts + h + 32, xb);
+            tm_wait_ld();
+            pin32(xa);
+            pin32(xb);
+            if (edge) { tc_hide(a, s, row, pos + h, fa); tc_hide(a, s, row, pos + h + 32, fb); }
+            mx = fmaxf(mx, fmaxf(tc_max(fa), tc_max(fb)));
+        }
+        tm_ld32(ts, xa);
+    }
+    mx *= c;
+    const bool grow = row.mine && mx > m + TC_LAZY;      // (from -inf: with the first visible position)
+    if (__any_sync(~0u, grow)) {
+        const float to_m = grow ? mx : m;
+        const float by = m == -INFINITY ? 0.f : ex2(m - to_m);
+        m = to_m;
+        l *= by;
+        // (this group's products so far are complete: they were issued before the scores)
+        if (!first) tc_rescale<D>(to, by);
+    }
+    const float off = (BF ? 0.f : 7.f) - (m == -INFINITY ? 0.f : m);
+    if (part >= 0) {
+        l += tc_exp16<BF>(fa, c, off, w);
+        tc_put_quarter(ts, part, w);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 128; h += 64) {
+            tm_wait_ld();
+            pin32(xa);
+            tm_ld32(ts + h + 32, xb);
+            if (edge) tc_hide(a, s, row, pos + h, fa);
+            l += tc_exp16<BF>(fa, c, off, w);
+            tm_st16(ts + h / 2, w);
+            tm_wait_ld();
+            pin32(xb);
+            if (h == 0) tm_ld32(ts + 64, xa);
+            if (edge) tc_hide(a, s, row, pos + h + 32, fb);
+            l += tc_exp16<BF>(fb, c, off, w);
+            tm_st16(ts + h / 2 + 16, w);
+        }
+    }
+    tm_wait_st();
+}
+
+// The same for 32-bit rows: weights as two f16 parts, the maximum moves with every block; returns what that makes of the sums so far.
+__device__ __forceinline__ float tc_weights32(const AttendParams &a, const SeqRows &s, const TcRow &row, uint32_t ts, int part, int pos, float c, float &m, float &l) {
+    uint32_t x[32], hi[16], lw[64];
+    float *const f = (float *)x;
+    const int p0 = part < 0 ? pos : pos + part * 32;
+    const bool edge = row.odd || __any_sync(~0u, row.mine && (p0 < row.lo || p0 + (part < 0 ? 128 : 32) > row.hi));
+    float mx = -INFINITY;
+    if (part >= 0) {
+        tm_ld(ts + part * 32, x);
+        if (edge) tc_hide(a, s, row, p0, f);
+        mx = tc_max(f);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 128; h += 32) {
+            tm_ld(ts + h, x);
+            if (edge) tc_hide(a, s, row, pos + h, f);
+            mx = fmaxf(mx, tc_max(f));
+        }
+    }
+    const float to_m = fmaxf(m, mx * c);
+    const float by = m == -INFINITY ? 0.f : ex2(m - to_m);
+    m = to_m;
+    l *= by;
+    const float off = m == -INFINITY ? 0.f : -m;
+    if (part >= 0) {
+        l += tc_exp32(f, c, off, hi, lw);
+        tc_put_quarter(ts, part, hi);
+        tc_put_quarter(ts + 64, part, lw);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 128; h += 32) {
+            tm_ld(ts + h, x);
+            if (edge) tc_hide(a, s, row, pos + h, f);
+            l += tc_exp32(f, c, off, hi, lw + h / 2);
+            tm_st16(ts + h / 2, hi);
+        }
+        tm_st32(ts + 64, lw);   // (over scores: only once all have been read)
+        tm_st32(ts + 96, lw + 32);
+    }
+    tm_wait_st();
+    return by;
+}
+
+// Four values of a finished row.
+template <int TY>
+__device__ __forceinline__ void put4(void *out, long long at, float4 y) {
+    if constexpr (TY == PTY_F32) *(float4 *)((float *)out + at) = y;
+    else *(uint2 *)((uint16_t *)out + at) = make_uint2(pack16<TY == PTY_BF16>(y.x, y.y), pack16<TY == PTY_BF16>(y.z, y.w));
+}
 
 template <int D, int TY>
 __global__ void __launch_bounds__(TC_THREADS, 1)
@@ -297,308 +506,332 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
     TcShared &sh = *(TcShared *)(ring + TC_STAGES * TILE);
     const AttendParams &a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const TcGeom g = tc_geom(a);
+    const int tq = 128 / a.group;
 
+    pdl_launch_dependents();   // (attend_join_kernel waits for this grid's end)
     if (tid == 0) {
         for (int i = 0; i < TC_STAGES; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
-        mbar_init(&sh.q_full, 8);
+        for (int i = 0; i < TC_SEGS; ++i) { mbar_init(&sh.seg_full[i], 1); mbar_init(&sh.seg_empty[i], 10); }
         for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 4); mbar_init(&sh.o_full[i], 1); mbar_init(&sh.o_free[i], 4); }
+        mbar_init(&sh.q_full, 8);
+        mbar_init(&sh.both, 8);
+        mbar_init(&sh.half, 4);
         mbar_init(&sh.drain, 1);
         sh.dead = sh.odd = 0;
+        for (int i = 0; i < 16; ++i) sh.gone[i >> 3][i & 7] = 0;
         fence_mbar_init();
     }
     if (warp == 9) tm_alloc(&sh.tmem, 512);
-
-    // units of every sequence, then their running sum
-    {
-        const int n = a.B.n;
-        const bool lanes = n < 64;  // few sequences: a warp each, its lanes over the tiles; many: a thread each
-        for (int i = lanes ? warp : tid; i < n; i += lanes ? TC_THREADS / 32 : TC_THREADS) {
-            TcTile x;
-            x.s = batch_seq(a.P, a.B, i);
-            const int nt = (x.s.rows + g.step - 1) / g.step;
-            int units = 0;
-            for (x.t = lanes ? lane : 0; x.t < nt; x.t += lanes ? 32 : 1) {
-                tc_span(a, g, x);
-                units = min(units + x.nb + TC_OVERHEAD, TC_MOST);
-            }
-            if (lanes)
-                for (int o = 16; o; o >>= 1) units = min(units + __shfl_xor_sync(~0u, units, o), TC_MOST);
-            if (!lanes || lane == 0) sh.prefix[i + 1] = (int)min((long long)units * a.P.kv, (long long)TC_MOST);
-        }
-        __syncthreads();
-        if (warp == 0) {
-            int run = 0;
-            for (int i0 = 0; i0 < n; i0 += 32) {
-                int v = i0 + lane < n ? sh.prefix[i0 + lane + 1] : 0;
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int y = __shfl_up_sync(~0u, v, o);
-                    if (lane >= o) v = min(v + y, TC_MOST);
-                }
-                v = min(run + v, TC_MOST);
-                if (i0 + lane < n) sh.prefix[i0 + lane + 1] = v;
-                run = __shfl_sync(~0u, v, 31);
-            }
-            if (lane == 0) sh.prefix[0] = 0;
-        }
-        __syncthreads();
-    }
-    // (offsets that overlap could claim more rows than there are: such a batch is left alone)
-    const int total = sh.prefix[a.B.n] < TC_MOST ? sh.prefix[a.B.n] : 0;
-    const int per = max((int)(((long long)total + p.n_ctas - 1) / p.n_ctas), TC_MIN_UNITS);
-    const int cta = blockIdx.x;
-    if (tid == 0 || tid == 32) {
-        const long long u = (long long)(cta + (tid ? 1 : 0)) * per;
-        tc_cut(a, g, sh.prefix, total, (int)(u < total ? u : total), tid ? sh.end : sh.begin);
-    }
+    for (int i = tid; i < min(a.B.n, TC_INFO); i += TC_THREADS) sh.info[i] = batch_seq(a.P, a.B, i);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    const int cta = blockIdx.x;
     const uint32_t tmem = sh.tmem;
     const uint32_t idesc_qk = tc_idesc(BF, 128, 128, false), idesc_pv = tc_idesc(BF, 128, D, true);
+    int ring0 = 0, n_seg = 0;             // ring entries before this segment, segments so far
+    bool ok = true;
+    auto segment = [&]() -> const TcSegment & { return sh.seg[n_seg % TC_SEGS]; };
+    auto seg_wait = [&] { return tc_wait(sh, &sh.seg_full[n_seg % TC_SEGS], (n_seg / TC_SEGS) & 1, p, 10); };
 
     // Register shares of the three groups of four warps: 2 x 208 + 80 <= 3 x 168, what the block was launched with.
-    TcWalk &wk = sh.walk[min(warp, 9)];
-    auto step = [&](bool first) {   // to the warp's first or next segment
-        __syncwarp();
-        int more = 0;
-        if (lane == 0) more = first ? wk.start(a, g, sh.begin, sh.end) : wk.next(a, g, sh.end);
-        __syncwarp();
-        return __shfl_sync(~0u, more, 0) != 0;
-    };
-    int ring0 = 0;                        // ring entries before this segment
-
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (warp == 8) {
-        // ------------------------------------------------------------------ TMA
-        const int boxes = max(1, TC_BLOCK >> a.P.shift), rows = min(a.P.page, TC_BLOCK);
-        bool ok = true;
-        int filled = 0;
-        for (bool more = step(true); more; more = step(false)) {
-            const int n = wk.j1 - wk.j0;
-            const bool wide = wk.x.ntok > g.tq;
-            for (int e = 0; e < 2 * n; ++e) {
-                // entry e of the segment: a block of K or of V
-                bool is_v;
-                int j;
-                if (wide) { is_v = e & 1; j = e >> 1; }
-                else if (e < 2 && e < n) { is_v = false; j = e; }
-                else if (e == 2 * n - 1) { is_v = true; j = n - 1; }
-                else { is_v = !(e & 1); j = is_v ? (e - 2) >> 1 : (e + 1) >> 1; }
-                const int pos = (wk.x.k0 + wk.j0 + j) * TC_BLOCK;
-                const int idx = ring0 + e, st = idx % TC_STAGES;
-                // a page that does not exist (or lies behind the sequence) is asked for outside the pool: zeros arrive
-                const int box = lane / PANELS, panel = lane % PANELS;
-                const int at = pos + box * rows;
-                int pg = a.P.n_pages;
-                if (box < boxes && at < wk.x.s.len) {
-                    pg = page_of(a.P, wk.x.s.slot, at);
-                    if (pg < 0) pg = a.P.n_pages;
+            // ------------------------------------------------------------------ TMA
+            const int box_shift = max(0, 7 - a.P.shift), boxes = 1 << box_shift, rows = min(a.P.page, TC_BLOCK), ahead = 32 >> box_shift;
+            const int box = lane / PANELS, panel = lane % PANELS;
+            int filled = 0;
+            while ((ok = __all_sync(~0u, seg_wait()))) {
+                const TcSegment &x = segment();
+                const int n = x.n;
+                if (n < 0) break;
+                const bool wide = x.ntok > tq;
+                // page numbers of `ahead` blocks from block from[.] on, one a lane; K and V move through them apart.  A page that does
+                // not exist (or lies behind the sequence) is asked for outside the pool: zeros arrive
+                int from[2] = {INT_MIN, INT_MIN}, pages[2];
+#pragma unroll 1
+                for (int e = 0; e < 2 * n; ++e) {
+                    // entry e of the segment: a block of K or of V
+                    bool is_v;
+                    int j;
+                    if (wide) { is_v = e & 1; j = e >> 1; }
+                    else if (e < 2 && e < n) { is_v = false; j = e; }
+                    else if (e == 2 * n - 1) { is_v = true; j = n - 1; }
+                    else { is_v = !(e & 1); j = is_v ? (e - 2) >> 1 : (e + 1) >> 1; }
+                    const int pos = (x.first + j) * TC_BLOCK;
+                    const int idx = ring0 + e, st = idx % TC_STAGES;
+                    int pg = 0;
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv)
+                        if (kv == (int)is_v) {
+                            if (from[kv] == INT_MIN || j >= from[kv] + ahead) {
+                                from[kv] = j;
+                                const int at = pos + (lane >> box_shift) * TC_BLOCK + (lane & (boxes - 1)) * rows;
+                                pages[kv] = at < x.s.len ? page_of(a.P, x.s.slot, at) : -1;
+                                if (pages[kv] < 0) pages[kv] = a.P.n_pages;
+                            }
+                            pg = __shfl_sync(~0u, pages[kv], ((j - from[kv]) << box_shift) + min(box, boxes - 1));
+                        }
+                    ok = __all_sync(~0u, tc_wait(sh, &sh.empty[st], ((idx / TC_STAGES) & 1) ^ 1, p, 1));
+                    if (!ok) break;
+                    filled = idx + 1;
+                    uint8_t *dst = ring + st * TILE;
+                    if (lane == 0) mbar_arrive_expect_tx(&sh.full[st], TILE);
+                    __syncwarp();
+                    if (box < boxes)
+                        tma_load_4d(dst + panel * (TC_BLOCK * 128) + box * rows * 128, is_v ? &vmap : &kmap, panel * 64, (pos + box * rows) & (a.P.page - 1), x.h, pg,
+                                    &sh.full[st]);
                 }
-                ok = __all_sync(~0u, tc_wait(sh, &sh.empty[st], ((idx / TC_STAGES) & 1) ^ 1, p, 1));
                 if (!ok) break;
-                filled = idx + 1;
-                uint8_t *dst = ring + st * TILE;
-                if (lane == 0) mbar_arrive_expect_tx(&sh.full[st], TILE);
+                ring0 += 2 * n;
                 __syncwarp();
-                if (box < boxes)
-                    tma_load_4d(dst + panel * (TC_BLOCK * 128) + box * rows * 128, is_v ? &vmap : &kmap, panel * 64, at & (a.P.page - 1), wk.x.h, pg, &sh.full[st]);
+                if (lane == 0) mbar_arrive(&sh.seg_empty[n_seg % TC_SEGS]);
+                ++n_seg;
             }
-            if (!ok) break;
-            ring0 += 2 * n;
-        }
-        // every copy that was asked for has arrived before the block ends
-        for (int idx = max(0, filled - TC_STAGES); idx < filled; ++idx)
-            (void)mbar_wait_bounded(&sh.full[idx % TC_STAGES], (idx / TC_STAGES) & 1, p.wait_limit);
-    } else if (warp == 9) {
-        // -------------------------------------------------------- tensor instructions: one thread
-        if (lane == 0) {
-            uint32_t ph_q = 0, ph_p[2] = {0, 0};
-            bool ok = true;
+            // every copy that was asked for has arrived before the block ends
+            for (int idx = max(0, filled - TC_STAGES); idx < filled; ++idx)
+                (void)mbar_wait_bounded(&sh.full[idx % TC_STAGES], (idx / TC_STAGES) & 1, p.wait_limit);
+        } else if (warp == 9 && lane == 0) {
+            // -------------------------------------------------------- tensor instructions: one thread
+            uint32_t ph_q = 0, ph_p = 0;
             const uint32_t q_addr = smem_u32(qs), r_addr = smem_u32(ring);
-            auto qk = [&](int w, int tile, int st) {
-                const uint32_t qa = q_addr + tile * TILE, ka = r_addr + st * TILE;
-                // (low parts first: a sum is truncated where it is, and theirs are small)
-#pragma unroll
-                for (int part = PARTS - 1; part >= 0; --part)
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t off = (k >> 2) * (TC_BLOCK * 128) + (k & 3) * 32;
-                        tc_mma_ss(tmem + w * 128, tc_desc(qa + part * TILE + off, 16), tc_desc(ka + off, 16), idesc_qk, part < PARTS - 1 || k > 0);
-                    }
-                tc_commit(&sh.s_full[w]);
-            };
-            auto pv = [&](int w, int st, bool add) {
-                const uint32_t va = r_addr + st * TILE;
-#pragma unroll
-                for (int part = PARTS - 1; part >= 0; --part)
-#pragma unroll
-                    for (int k = 0; k < TC_BLOCK / 16; ++k)
-                        tc_mma_ts(tmem + O_COL + w * D, tmem + w * 128 + part * 64 + k * 8, tc_desc(va + k * 2048, TC_BLOCK * 128), idesc_pv,
-                                  add || part < PARTS - 1 || k > 0);
-            };
-            auto full = [&](int idx) { return tc_wait(sh, &sh.full[idx % TC_STAGES], (idx / TC_STAGES) & 1, p, 2); };
-            auto weights = [&](int w) {
-                const bool r = tc_wait(sh, &sh.p_full[w], ph_p[w], p, 3);
-                ph_p[w] ^= 1;
-                tc_fence_after();
-                return r;
-            };
-            for (bool more = wk.start(a, g, sh.begin, sh.end); ok && more; more = wk.next(a, g, sh.end)) {
-                const int n = wk.j1 - wk.j0;
+            while ((ok = seg_wait())) {
+                const int n = segment().n;
+                if (n < 0) break;
+                const bool wide = !F32 && segment().ntok > tq;
+                mbar_arrive(&sh.seg_empty[n_seg % TC_SEGS]);
+                ++n_seg;
                 if (n == 0) continue;
-                const bool wide = wk.x.ntok > g.tq;
                 if (!(ok = tc_wait(sh, &sh.q_full, ph_q, p, 4))) break;
                 ph_q ^= 1;
-                if (!F32 && wide) {
-                    if (!(ok = full(ring0))) break;
-                    tc_fence_after();
-                    qk(0, 0, ring0 % TC_STAGES);
-                    qk(1, 1, ring0 % TC_STAGES);
-                    tc_commit(&sh.empty[ring0 % TC_STAGES]);
-                    for (int j = 0; j < n; ++j) {
-                        const int v = ring0 + 2 * j + 1, kn = v + 1;
-                        if (!(ok = full(v) && weights(0))) break;
-                        pv(0, v % TC_STAGES, j > 0);
-                        if (j + 1 < n) {
-                            if (!(ok = full(kn))) break;
-                            tc_fence_after();
-                            qk(0, 0, kn % TC_STAGES);
-                        } else {
-                            tc_commit(&sh.o_full[0]);
-                        }
-                        if (!(ok = weights(1))) break;
-                        pv(1, v % TC_STAGES, j > 0);
-                        tc_commit(&sh.empty[v % TC_STAGES]);
-                        if (j + 1 < n) {
-                            qk(1, 1, kn % TC_STAGES);
-                            tc_commit(&sh.empty[kn % TC_STAGES]);
-                        } else {
-                            tc_commit(&sh.o_full[1]);
-                        }
-                    }
-                } else {
-                    for (int j = 0; j < 2 && j < n; ++j) {
-                        if (!(ok = full(ring0 + j))) break;
+                // Step i is the product with V of one group and the scores of its next block: wide, both groups for every block (group
+                // i & 1, block i / 2); narrow, the groups in turn (block i).  The first two steps have scores only.
+                const int steps = wide ? 2 * n : n;
+                for (int i = -2; i < steps; ++i) {
+                    const int w = i & 1;
+                    const bool last = i + 2 >= steps, both = !wide || w;   // both: no other group needs the block any more
+                    if (i >= 0) {
+                        const int v = ring0 + tc_slot_v(wide, wide ? i >> 1 : i, n), st = v % TC_STAGES;
+                        if (!(ok = tc_wait(sh, &sh.full[st], (v / TC_STAGES) & 1, p, 2) && tc_wait(sh, &sh.p_full[w], ph_p >> w & 1, p, 3))) break;
+                        ph_p ^= 1u << w;
                         tc_fence_after();
-                        qk(j, 0, (ring0 + j) % TC_STAGES);
-                        tc_commit(&sh.empty[(ring0 + j) % TC_STAGES]);
+                        const uint32_t va = r_addr + st * TILE;
+                        const bool add = !F32 && i > 1;
+#pragma unroll
+                        for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                            for (int k = 0; k < TC_BLOCK / 16; ++k)
+                                tc_mma_ts(tmem + O_COL + w * D, tmem + w * 128 + part * 64 + k * 8, tc_desc(va + k * 2048, TC_BLOCK * 128), idesc_pv,
+                                          add || part < PARTS - 1 || k > 0);
+                        if (both) tc_commit(&sh.empty[st]);
+                        if (F32 || last) tc_commit(&sh.o_full[w]);
                     }
-                    for (int j = 0; ok && j < n; ++j) {
-                        const int w = j & 1, v = ring0 + tc_slot_v(false, j, n), kn = ring0 + tc_slot_k(false, j + 2);
-                        if (!(ok = full(v) && weights(w))) break;
-                        pv(w, v % TC_STAGES, !F32 && j > 1);
-                        tc_commit(&sh.empty[v % TC_STAGES]);
-                        if (F32) tc_commit(&sh.o_full[w]);
-                        if (j + 2 < n) {
-                            if (!(ok = full(kn))) break;
-                            tc_fence_after();
-                            qk(w, 0, kn % TC_STAGES);
-                            tc_commit(&sh.empty[kn % TC_STAGES]);
-                        } else if (!F32) {
-                            tc_commit(&sh.o_full[w]);
-                        }
+                    if (!last) {
+                        const int kn = ring0 + tc_slot_k(wide, wide ? (i + 2) >> 1 : i + 2), st = kn % TC_STAGES;
+                        if (!(ok = tc_wait(sh, &sh.full[st], (kn / TC_STAGES) & 1, p, 2))) break;
+                        tc_fence_after();
+                        const uint32_t qa = q_addr + (wide ? w * TILE : 0), ka = r_addr + st * TILE;
+                        // (low parts first: a sum is truncated where it is, and theirs are small)
+#pragma unroll
+                        for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                            for (int k = 0; k < D / 16; ++k) {
+                                const uint32_t off = (k >> 2) * (TC_BLOCK * 128) + (k & 3) * 32;
+                                tc_mma_ss(tmem + w * 128, tc_desc(qa + part * TILE + off, 16), tc_desc(ka + off, 16), idesc_qk, part < PARTS - 1 || k > 0);
+                            }
+                        tc_commit(&sh.s_full[w]);
+                        if (both) tc_commit(&sh.empty[st]);
                     }
                 }
+                if (!ok) break;
                 ring0 += 2 * n;
+            }
+        } else if (warp == 10) {
+            // ------------------------------------------------------- units of every sequence, their running sum, the CTA's segments
+            const TcBatch g(a, sh.info);
+            const int seqs = a.B.n;
+            const bool lanes = seqs < 32;  // few sequences: the lanes over a sequence's tiles; many: a lane each
+            int total = 0;
+            if (lane == 0) sh.prefix[0] = 0;
+#pragma unroll 1
+            for (int i0 = 0; i0 < seqs; i0 += lanes ? 1 : 32) {
+                const int i = lanes ? i0 : i0 + lane;
+                int units = 0;
+                if (i < seqs) {
+                    TcTile x;
+                    x.s = g.seq(i);
+                    const int nt = (x.s.rows + g.step - 1) / g.step;
+#pragma unroll 1
+                    for (x.t = lanes ? lane : 0; x.t < nt; x.t += lanes ? 32 : 1) {
+                        tc_span(g, x);
+                        units = min(units + x.nb + TC_OVERHEAD, TC_MOST);
+                    }
+                }
+                if (lanes)
+                    for (int o = 16; o; o >>= 1) units = min(units + __shfl_xor_sync(~0u, units, o), TC_MOST);
+                units = (int)min((long long)units * a.P.kv, (long long)TC_MOST);
+                if (!lanes)
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int y = __shfl_up_sync(~0u, units, o);
+                        if (lane >= o) units = min(units + y, TC_MOST);
+                    }
+                units = min(total + units, TC_MOST);
+                if (i < seqs && (!lanes || lane == 0)) sh.prefix[i + 1] = units;
+                total = __shfl_sync(~0u, units, 31);
+            }
+            __syncwarp();
+            // (offsets that overlap could claim more rows than there are: such a batch is left alone)
+            if (total >= TC_MOST) total = 0;
+            const int per = max((int)(((long long)total + p.n_ctas - 1) / p.n_ctas), TC_MIN_UNITS);
+            if (lane < 2) {
+                const long long u = (long long)(cta + lane) * per;
+                tc_cut(g, sh.prefix, total, (int)(u < total ? u : total), sh.cut[lane]);
+            }
+            __syncwarp();
+            if (lane == 0) {
+                TcWalk wk;
+                int cuts = 0;
+                bool more = wk.start(g, sh.cut[0], sh.cut[1]);
+#pragma unroll 1
+                for (;;) {
+                    const int at = n_seg % TC_SEGS;
+                    if (!tc_wait(sh, &sh.seg_empty[at], ((n_seg / TC_SEGS) & 1) ^ 1, p, 11)) break;
+                    TcSegment &x = sh.seg[at];
+                    x.s = wk.x.s;
+                    x.h = wk.x.h; x.tok0 = wk.x.tok0; x.ntok = wk.x.ntok;
+                    x.first = wk.x.k0 + wk.j0;
+                    x.n = more ? wk.j1 - wk.j0 : -1;
+                    x.base = wk.x.base; x.nb = wk.x.nb; x.j0 = wk.j0;
+                    mbar_arrive(&sh.seg_full[at]);
+                    if (!more) break;
+                    // the first of a cut tile's pieces says how many follow: the cuts that stay inside the tile
+                    if (wk.j0 == 0 && wk.j1 < wk.x.nb) {
+                        const int lo = wk.x.base + TC_OVERHEAD + 2, hi = wk.x.base + TC_OVERHEAD + wk.x.nb - 2;
+                        int *mt = p.meta + cta * 8;
+                        cuts = hi / per - (lo - 1) / per;
+                        mt[1] = wk.x.s.first + wk.x.tok0; mt[2] = wk.x.ntok; mt[3] = wk.x.h; mt[4] = !F32 && wk.x.ntok > tq;
+                    }
+                    ++n_seg;
+                    more = wk.next(g, sh.cut[1]);
+                }
+                p.meta[cta * 8] = cuts;
             }
         }
         __syncwarp();
-        }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ------------------------------------------------------------------ softmax
-        // (after a wait that ran out the groups go on through their barriers, without the work)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int w = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // TMEM lane base of the warp, in the address's upper half
-        const uint32_t ts = tmem + lanes + w * 128, to = tmem + lanes + O_COL + w * D;
         const bool flip = a.scale_log2 < 0.f;                // a negative scale turns the queries round
-        const float c = fmaxf(fabsf(a.scale_log2), 1e-30f);  // (a scale of 0: hidden positions still get 2^-inf)
-        const float shift = BF ? 0.f : 7.f;
-        uint32_t ph_s = 0, ph_b = 0, ph_o[2] = {0, 0};
-        bool ok = true, meta = false;
-        auto wait = [&](uint64_t *bar, uint32_t parity, int site) { ok = __all_sync(~0u, ok && tc_wait(sh, bar, parity, p, site)); return ok; };
-        for (bool more = step(true); more; more = step(false)) {
-            const TcTile &x = wk.x;
-            const int n = wk.j1 - wk.j0, k_first = x.k0 + wk.j0;
-            const bool wide = x.ntok > g.tq;
-            const bool whole = wk.j0 == 0 && wk.j1 == x.nb;
-            // the row that this thread looks after
-            const int tok = x.tok0 + (wide ? w * g.tq : 0) + r / a.group;
-            const bool mine = r < g.tq * a.group && tok < x.tok0 + x.ntok;
-            const int row = x.s.first + tok, head = x.h * a.group + r % a.group;
-            int lo = 0, hi = 0;
-            if (mine) row_span(a, x.s.len, x.s.len - x.s.rows + tok, lo, hi);
+        const float c0 = fmaxf(fabsf(a.scale_log2), 1e-30f); // (a scale of 0: hidden positions still get 2^-inf)
+        uint32_t ph_s = 0, ph_b = 0, ph_o = 0, ph_both = 0, ph_half = 0;
+        auto wait = [&](uint64_t *bar, uint32_t parity, int site) { return ok = __all_sync(~0u, tc_wait(sh, bar, parity, p, site)); };
+        // both groups, or the four warps of one, wait for one another (as bounded as any other wait)
+        auto meet = [&](uint64_t *bar, uint32_t &ph, int site) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+            const bool k = wait(bar, ph, site);
+            ph ^= 1;
+            return k;
+        };
+        while (wait(&sh.seg_full[n_seg % TC_SEGS], (n_seg / TC_SEGS) & 1, 10)) {
+            const TcSegment &x = segment();
+            const int n = x.n, k_first = x.first;
+            if (n < 0) break;
+            const bool wide = !F32 && x.ntok > tq;
+            const bool whole = n == x.nb;
+            // Up to 32 rows are held four times over and every copy weighs a quarter of a block's positions: four warps then work on
+            // what one would.
+            const int held = min(x.ntok, tq) * a.group;
+            const int each = wide || held > 32 ? 128 : 32, reps = 128 / each;
+            const int rr = r & (each - 1), part = reps > 1 ? r >> 5 : -1;   // the thread's row and quarter
+            const int tok = x.tok0 + (wide ? w * tq : 0) + rr / a.group;
+            TcRow row;
+            row.mine = rr < tq * a.group && tok < x.tok0 + x.ntok;
+            const int out_row = x.s.first + tok, head = x.h * a.group + rr % a.group;
+            row.lo = row.hi = 0;
+            if (row.mine) row_span(a, x.s.len, x.s.len - x.s.rows + tok, row.lo, row.hi);
             // pages that are not there: looked for once a segment
             bool odd = false;
-            for (int c0 = (k_first * TC_BLOCK >> a.P.shift) + tid; (c0 << a.P.shift) < min((k_first + n) * TC_BLOCK, x.s.len); c0 += 256)
-                odd |= page_of(a.P, x.s.slot, c0 << a.P.shift) < 0;
-            odd = softmax_bar_or(odd);   // (also: both groups have left the segment before)
-            if (n > 0 && ok) {
-                const int rows = min(x.ntok, g.tq) * a.group;
-                const int tok_a = x.tok0 + (wide ? w * g.tq : 0);
-                const int n_rows = wide && w ? (x.ntok - g.tq) * a.group : rows;
-                const int nth = wide ? 128 : 256, me = wide ? r : tid;
-                uint8_t *q_tile = qs + (wide ? w * TILE : 0);
-                if constexpr (F32) {
-                    constexpr int E = D / 32;
-                    for (int rr = warp; rr < n_rows; rr += 8) {
-                        const float *src = (const float *)a.q + (long long)(x.s.first + tok_a + rr / a.group) * a.qs[0] +
-                                           (long long)(x.h * a.group + rr % a.group) * a.qs[1] + lane * E;
-                        float v[E], mx = 0.f;
+            #pragma unroll 1
+            for (int c = (k_first * TC_BLOCK >> a.P.shift) + tid; (c << a.P.shift) < min((k_first + n) * TC_BLOCK, x.s.len); c += 256)
+                odd |= page_of(a.P, x.s.slot, c << a.P.shift) < 0;
+
+            // ---- queries into shared memory, four loads at a time; the first are on their way before the groups meet
+            const int q_rows = wide && w ? (x.ntok - tq) * a.group : held;
+            const long long q_tok = x.s.first + x.tok0 + (wide ? w * tq : 0);
+            uint8_t *const q_tile = qs + (wide ? w * TILE : 0);
+            constexpr int E = F32 ? D / 32 : 8;              // values of a load: a row per warp, or 16 bytes
+            const int q_units = n == 0 ? 0 : (F32 ? q_rows : q_rows * (D / 8)), q_step = F32 ? 8 : (wide ? 128 : 256);
+            const int q_me = F32 ? warp : (wide ? r : tid);
+            uint4 qv[4];
+            auto q_load = [&](int i0) {
 #pragma unroll
-                        for (int e = 0; e < E; ++e) { v[e] = src[e]; mx = fmaxf(mx, fabsf(v[e])); }
-                        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
-                        // the row's largest value lands in [2^13, 2^14): what is 2^-27 of it still has 11 bits
-                        const int ex = mx < INFINITY ? max((int)(__float_as_uint(mx) >> 23) - 127, -100) : 0;
-                        const float by = __uint_as_float((uint32_t)(127 + 13 - ex) << 23) * (flip ? -1.f : 1.f);
-                        if (lane == 0) sh.unit[rr] = __uint_as_float((uint32_t)max(127 - 13 + ex, 1) << 23);
+                for (int u = 0; u < 4; ++u) {
+                    const int i = i0 + u * q_step;
+                    if (i >= q_units) break;
+                    const int rw = F32 ? i : i / (D / 8), d = F32 ? lane * E : (i % (D / 8)) * 8;
+                    const long long at = (q_tok + rw / a.group) * a.qs[0] + (long long)(x.h * a.group + rw % a.group) * a.qs[1] + d;
+                    if constexpr (!F32) qv[u] = *(const uint4 *)((const uint16_t *)a.q + at);
+                    else if constexpr (D == 128) qv[u] = *(const uint4 *)((const float *)a.q + at);
+                    else *(uint2 *)&qv[u] = *(const uint2 *)((const float *)a.q + at);
+                }
+            };
+            q_load(q_me);
+            if (__any_sync(~0u, odd) && lane == 0) sh.gone[n_seg & 1][warp] = 1;
+            if (!meet(&sh.both, ph_both, 12)) break;   // (both groups have left the segment before)
+            row.odd = false;
+            for (int i = 0; i < 8; ++i) row.odd |= sh.gone[n_seg & 1][i] != 0;
+            if (lane == 0) sh.gone[(n_seg & 1) ^ 1][warp] = 0;
+            if (n > 0) {
+#pragma unroll 1
+                for (int i0 = q_me; i0 < q_units; i0 += 4 * q_step) {
+                    if (i0 > q_me) q_load(i0);
 #pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            const float u0 = v[e] * by, u1 = v[e + 1] * by;
-                            const uint32_t hi = pack16<false>(u0, u1);
-                            const float2 h = unpack16(hi);
-                            const int d = lane * E + e;
-                            uint8_t *at = q_tile + (d >> 6) * (TC_BLOCK * 128) + sw128(rr, (d >> 3) & 7) + (d & 7) * 2;
-                            *(uint32_t *)at = hi;
-                            *(uint32_t *)(at + TILE) = pack16<false>(u0 - h.x, u1 - h.y);
+                    for (int u = 0; u < 4; ++u) {
+                        const int i = i0 + u * q_step;
+                        if (i >= q_units) break;
+                        if constexpr (F32) {
+                            const float *v = (const float *)&qv[u];
+                            float mx = 0.f;
+#pragma unroll
+                            for (int e = 0; e < E; ++e) mx = fmaxf(mx, fabsf(v[e]));
+                            for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+                            // the row's largest value lands in [2^13, 2^14): what is 2^-27 of it still has 11 bits
+                            const int ex = mx < INFINITY ? max((int)(__float_as_uint(mx) >> 23) - 127, -100) : 0;
+                            const float by = __uint_as_float((uint32_t)(127 + 13 - ex) << 23) * (flip ? -1.f : 1.f);
+                            if (lane == 0) sh.unit[i] = __uint_as_float((uint32_t)max(127 - 13 + ex, 1) << 23);
+#pragma unroll
+                            for (int e = 0; e < E; e += 2) {
+                                const float u0 = v[e] * by, u1 = v[e + 1] * by;
+                                const uint32_t hi = pack16<false>(u0, u1);
+                                const float2 h = unpack16(hi);
+                                const uint32_t lw = pack16<false>(u0 - h.x, u1 - h.y);
+                                const int d = lane * E + e;
+                                for (int c = 0; c < reps; ++c) {
+                                    uint8_t *at = q_tile + (d >> 6) * (TC_BLOCK * 128) + sw128(i + c * each, (d >> 3) & 7) + (d & 7) * 2;
+                                    *(uint32_t *)at = hi;
+                                    *(uint32_t *)(at + TILE) = lw;
+                                }
+                            }
+                        } else {
+                            uint4 v = qv[u];
+                            if (flip) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
+                            const int rw = i / (D / 8), ch = i % (D / 8);
+                            for (int c = 0; c < reps; ++c) *(uint4 *)(q_tile + (ch >> 3) * (TC_BLOCK * 128) + sw128(rw + c * each, ch & 7)) = v;
                         }
                     }
-                } else
-                for (int i = me; i < n_rows * (D / 8); i += nth) {
-                    const int rr = i / (D / 8), ch = i % (D / 8);
-                    const uint16_t *src = (const uint16_t *)a.q + (long long)(x.s.first + tok_a + rr / a.group) * a.qs[0] +
-                                          (long long)(x.h * a.group + rr % a.group) * a.qs[1] + ch * 8;
-                    uint4 v = *(const uint4 *)src;
-                    if (flip) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
-                    *(uint4 *)(q_tile + (ch >> 3) * (TC_BLOCK * 128) + sw128(rr, ch & 7)) = v;
                 }
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.q_full);
             }
+
+            // ---- blocks
             float m = -INFINITY, l = 0.f;   // m: of the scaled scores, what the weights refer to
-            const bool warp_mine = __any_sync(~0u, mine);
-            // scores of positions that the row does not see
-            auto hide = [&](float *f, int pos) {
-                                    if (odd || __any_sync(~0u, mine && (pos < lo || pos + TC_BLOCK > hi))) {
-                                        uint32_t see[4];   // a bit per position
-                #pragma unroll
-                                        for (int k = 0; k < 4; ++k) see[k] = bits_below(hi - pos - 32 * k) & ~bits_below(lo - pos - 32 * k);
-                                        if (odd)
-                                            for (int at = pos; at < min(pos + TC_BLOCK, x.s.len); at += min(a.P.page, 32))
-                                                if (page_of(a.P, x.s.slot, at) < 0) {
-                                                    const uint32_t gone = bits_below(min(a.P.page, 32)) << (at & 31);
-                #pragma unroll
-                                                    for (int k = 0; k < 4; ++k)
-                                                        if (((at - pos) >> 5) == k) see[k] &= ~gone;
-                                                }
-                #pragma unroll
-                                        for (int k = 0; k < 128; ++k)
-                                            if (!((see[k >> 5] >> (k & 31)) & 1u)) f[k] = -INFINITY;
-                                    }
-            };
+            const bool warp_mine = __any_sync(~0u, row.mine);
             // What lies behind the sequence in its last page takes part in the product with weight 0: it may not be NaN.
             auto clear_tail = [&](int j, int pos) {
                 const int idx = ring0 + tc_slot_v(wide, j, n);
@@ -611,10 +844,47 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                 fence_async_smem();
                 return true;
             };
-            const int slot = 2 * cta + (wk.j0 == 0 ? 1 : 0);
+            const int slot = 2 * cta + (x.j0 == 0 ? 1 : 0);
+            float *const scratch = (float *)qs;   // [128][D], once a segment's queries have done their work: 16-byte chunks swizzled by the row
+            // A narrow tile's results go through the scratch: 32 values of the thread's own row, relative to `top` with the weights' sum lt.
+            auto put_scratch = [&](int h, const float *f) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) ((float4 *)scratch)[r * (D / 4) + (((h + k) / 4) ^ (rr & (D / 4 - 1)))] = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
+            };
+            // ... and the 128 threads of a group join the copies and write the rows, or a piece of them.
+            auto join_copies = [&](float top_, float lt_) {
+                sh.red[r][0] = top_;
+                sh.red[r][1] = lt_;
+                if (!meet(&sh.half, ph_half, 13)) return;
+#pragma unroll 1
+                for (int i = r; i < held * (D / 4); i += 128) {
+                    const int rw = i / (D / 4), ch = i % (D / 4);
+                    float top = -INFINITY, lt = 0.f;
+#pragma unroll 1
+                    for (int q = 0; q < reps; ++q) top = fmaxf(top, sh.red[q * each + rw][0]);
+                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                    for (int q = 0; q < reps; ++q) {
+                        const float mq = sh.red[q * each + rw][0], b = mq == -INFINITY ? 0.f : ex2(mq - top);
+                        const float4 o = ((const float4 *)scratch)[(q * each + rw) * (D / 4) + (ch ^ (rw & (D / 4 - 1)))];
+                        lt += sh.red[q * each + rw][1] * b;
+                        y.x = fmaf(o.x, b, y.x); y.y = fmaf(o.y, b, y.y); y.z = fmaf(o.z, b, y.z); y.w = fmaf(o.w, b, y.w);
+                    }
+                    if (whole) {
+                        const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
+                        y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
+                        if (!(fabsf(y.x) + fabsf(y.y) + fabsf(y.z) + fabsf(y.w) < INFINITY)) sh.odd = 1;   // (see attend_join_kernel)
+                        put4<TY>(a.out, (long long)(x.s.first + x.tok0 + rw / a.group) * a.os[0] + (long long)(x.h * a.group + rw % a.group) * a.os[1] + ch * 4, y);
+                    } else {
+                        *(float4 *)(p.part + ((long long)slot * p.ws_rows + rw) * D + ch * 4) = y;
+                        if (ch == 0) *(float2 *)(p.ml + ((long long)slot * p.ws_rows + rw) * 2) = make_float2(top, lt);
+                    }
+                }
+            };
+
             if constexpr (F32) {
-                softmax_bar_or(false);   // the rows' powers of two are written
-                const float cr = c * sh.unit[r];
+                if (!meet(&sh.both, ph_both, 14)) break;   // the rows' powers of two are written
+                const float c = c0 * sh.unit[rr];
                 if (w == 0) {
                     for (int j = 0; j < n && ok; ++j) {
                         const int b = j & 1, pos = (k_first + j) * TC_BLOCK;
@@ -623,36 +893,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                         if (!wait(&sh.o_free[b], (ph_b >> b & 1) ^ 1, 9)) break;
                         ph_b ^= 1 << b;
                         tc_fence_after();
-                        if (warp_mine) {
-                            const uint32_t tb = tmem + lanes + b * 128;
-                            uint32_t s[128], hi[64], lw[64];
-                            tm_ld32(tb, s); tm_ld32(tb + 32, s + 32); tm_ld32(tb + 64, s + 64); tm_ld32(tb + 96, s + 96);
-                            tm_wait_ld();
-                            pin32(s); pin32(s + 32); pin32(s + 64); pin32(s + 96);
-                            float *f = (float *)s;
-                            hide(f, pos);
-                            float mx[4] = {f[0], f[1], f[2], f[3]};
-#pragma unroll
-                            for (int k = 4; k < 128; ++k) mx[k & 3] = fmaxf(mx[k & 3], f[k]);
-                            const float to_m = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * cr);
-                            const float by = m == -INFINITY ? 0.f : ex2(m - to_m);
-                            m = to_m;
-                            sh.by[b][r] = by;
-                            const float off = m == -INFINITY ? 0.f : -m;
-                            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                            for (int k = 0; k < 128; k += 2) {
-                                // weights up to 2^14 (f16 ends at 2^16); as a factor: in the exponent it would cost the argument bits
-                                const float p0 = 16384.f * ex2(fmaf(f[k], cr, off)), p1 = 16384.f * ex2(fmaf(f[k + 1], cr, off));
-                                sum[(k >> 1) & 3] += p0 + p1;
-                                hi[k >> 1] = pack16<false>(p0, p1);
-                                const float2 h = unpack16(hi[k >> 1]);
-                                lw[k >> 1] = pack16<false>(p0 - h.x, p1 - h.y);
-                            }
-                            l = l * by + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-                            tm_st32(tb, hi); tm_st32(tb + 32, hi + 32); tm_st32(tb + 64, lw); tm_st32(tb + 96, lw + 32);
-                            tm_wait_st();
-                        }
+                        if (warp_mine) sh.by[b][r] = tc_weights32(a, x.s, row, tmem + lanes + b * 128, part, pos, c, m, l);
                         if (pos + TC_BLOCK > x.s.len && !clear_tail(j, pos)) break;
                         tc_fence_before();
                         __syncwarp();
@@ -660,7 +901,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                     }
                     sh.ml[r][0] = m;
                     sh.ml[r][1] = l;
-                    softmax_bar_or(false);
+                    if (!ok || !meet(&sh.both, ph_both, 15)) break;
                 } else {
                     float acc[D];
 #pragma unroll
@@ -676,9 +917,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
 #pragma unroll
                             for (int h = 0; h < D; h += 32) {
                                 uint32_t o[32];
-                                tm_ld32(tmem + lanes + O_COL + b * D + h, o);
-                                tm_wait_ld();
-                                pin32(o);
+                                tm_ld(tmem + lanes + O_COL + b * D + h, o);
 #pragma unroll
                                 for (int k = 0; k < 32; ++k) acc[h + k] = fmaf(acc[h + k], by, __uint_as_float(o[k]));
                             }
@@ -687,164 +926,96 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sh.o_free[b]);
                     }
-                    softmax_bar_or(false);
-                    const float top = sh.ml[r][0], lt = sh.ml[r][1], inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
-                    float *dst = whole ? (float *)a.out + row * a.os[0] + head * a.os[1] : p.part + ((long long)slot * p.ws_rows + r) * D;
-                    float size = 0.f;
-                    if (mine && ok) {
+                    if (!ok || !meet(&sh.both, ph_both, 15)) break;
+                    if (row.mine) {
 #pragma unroll
-                        for (int k = 0; k < D; k += 4) {
-                            const float u = whole ? inv : 1.f;
-                            const float4 y = make_float4(acc[k] * u, acc[k + 1] * u, acc[k + 2] * u, acc[k + 3] * u);
-                            size += (fabsf(y.x) + fabsf(y.y)) + (fabsf(y.z) + fabsf(y.w));
-                            *(float4 *)(dst + k) = y;
-                        }
-                        if (!whole) *(float2 *)(p.ml + ((long long)slot * p.ws_rows + r) * 2) = make_float2(top, lt);
-                        else if (!(size < INFINITY)) sh.odd = 1;   // (see attend_join_kernel)
+                        for (int h = 0; h < D; h += 32) put_scratch(h, acc + h);
                     }
+                    join_copies(sh.ml[r][0], sh.ml[r][1]);
                 }
-                ring0 += 2 * n;
             } else {
-            const int cnt = wide ? n : (n - w + 1) >> 1;
-            for (int i = 0; i < cnt && ok; ++i) {
-                const int j = wide ? i : 2 * i + w, pos = (k_first + j) * TC_BLOCK;
-                if (!wait(&sh.s_full[w], ph_s, 5)) break;
-                ph_s ^= 1;
+                const uint32_t ts = tmem + lanes + w * 128, to = tmem + lanes + O_COL + w * D;
+                const int cnt = wide ? n : (n - w + 1) >> 1;
+                for (int i = 0; i < cnt && ok; ++i) {
+                    const int j = wide ? i : 2 * i + w, pos = (k_first + j) * TC_BLOCK;
+                    if (!wait(&sh.s_full[w], ph_s, 5)) break;
+                    ph_s ^= 1;
+                    tc_fence_after();
+                    if (warp_mine) tc_weights16<D, BF>(a, x.s, row, ts, to, part, pos, i == 0, c0, m, l);
+                    if (pos + TC_BLOCK > x.s.len && !clear_tail(j, pos)) break;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.p_full[w]);
+                }
+                // ---- the segment's result
+                float m1 = -INFINITY, l1 = 0.f;
+                const bool two = !wide && n > 1;
+                if (!wide) {
+                    if (w == 1) { sh.ml[r][0] = m; sh.ml[r][1] = l; }
+                    if (!ok || !meet(&sh.both, ph_both, 16)) break;
+                    if (w == 0) { m1 = sh.ml[r][0]; l1 = sh.ml[r][1]; }
+                }
+                if (!ok) break;
+                if (n > 0 && (wide || w == 0) && !wait(&sh.o_full[w], ph_o >> w & 1, 7)) break;
+                if (two && w == 0 && !wait(&sh.o_full[1], ph_o >> 1, 8)) break;
+                ph_o ^= (n > 0 ? 1u : 0u) | ((wide ? n > 0 : n > 1) ? 2u : 0u);
                 tc_fence_after();
-                if (warp_mine) {
-                    uint32_t s[128];
-                    tm_ld32(ts, s); tm_ld32(ts + 32, s + 32); tm_ld32(ts + 64, s + 64); tm_ld32(ts + 96, s + 96);
-                    tm_wait_ld();
-                    pin32(s); pin32(s + 32); pin32(s + 64); pin32(s + 96);
-                    float *f = (float *)s;
-                    hide(f, pos);
-                    float mx = f[0];
+                if (wide || w == 0) {
+                    const float top = fmaxf(m, m1);
+                    // (weights that refer to -inf are all 0, and their O holds zeros)
+                    const float b0 = m == -INFINITY ? 0.f : ex2(m - top), b1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
+                    const float lt = l * b0 + l1 * b1, inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt), u = wide && whole ? inv : b0;
+                    const long long ws_at = (long long)slot * p.ws_rows + w * 128 + r;
+                    if (warp_mine) {
+#pragma unroll 1
+                        for (int h = 0; h < D; h += 32) {
+                            uint32_t o[32];
+                            float *f = (float *)o;
+                            if (n > 0) {
+                                tm_ld(to + h, o);
+                            } else {
 #pragma unroll
-                    for (int k = 1; k < 128; ++k) mx = fmaxf(mx, f[k]);
-                    mx *= c;
-                    const bool grow = mx > m + TC_LAZY;      // (from -inf: with the first visible position)
-                    if (__any_sync(~0u, grow)) {
-                        const float to_m = grow ? mx : m;
-                        const float by = m == -INFINITY ? 0.f : ex2(m - to_m);
-                        m = to_m;
-                        l *= by;
-                        if (i > 0) {
-                            // this group's products so far are complete: they were issued before the scores
+                                for (int k = 0; k < 32; ++k) o[k] = 0;
+                            }
 #pragma unroll
-                            for (int h = 0; h < D; h += 32) {
-                                uint32_t o[32];
-                                tm_ld32(to + h, o);
-                                tm_wait_ld();
-                                pin32(o);
+                            for (int k = 0; k < 32; ++k) f[k] *= u;
+                            if (two) {
+                                uint32_t o1[32];
+                                tm_ld(to + D + h, o1);
 #pragma unroll
-                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
-                                tm_st32(to + h, o);
+                                for (int k = 0; k < 32; ++k) f[k] = fmaf(__uint_as_float(o1[k]), b1, f[k]);
+                            }
+                            if (!row.mine) continue;
+                            if (!wide) {
+                                put_scratch(h, f);
+                            } else if (whole) {
+                                float size = 0.f;
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) size += fabsf(f[k]);
+                                if (!(size < INFINITY)) sh.odd = 1;   // (see attend_join_kernel)
+                                uint16_t *out = (uint16_t *)a.out + out_row * a.os[0] + head * a.os[1] + h;
+#pragma unroll
+                                for (int k = 0; k < 32; k += 8)
+                                    *(uint4 *)(out + k) = make_uint4(pack16<BF>(f[k], f[k + 1]), pack16<BF>(f[k + 2], f[k + 3]), pack16<BF>(f[k + 4], f[k + 5]),
+                                                                     pack16<BF>(f[k + 6], f[k + 7]));
+                            } else {
+                                float *pt = p.part + ws_at * D + h;
+#pragma unroll
+                                for (int k = 0; k < 32; k += 4) *(float4 *)(pt + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
                             }
                         }
+                        if (wide && !whole && row.mine) *(float2 *)(p.ml + ws_at * 2) = make_float2(top, lt);
                     }
-                    const float off = shift - (m == -INFINITY ? 0.f : m);
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < 128; k += 2) {
-                        const float p0 = ex2(fmaf(f[k], c, off)), p1 = ex2(fmaf(f[k + 1], c, off));
-                        sum[(k >> 1) & 3] += p0 + p1;
-                        s[k >> 1] = pack16<BF>(p0, p1);
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tm_st32(ts, s);
-                    tm_st32(ts + 32, s + 32);
-                    tm_wait_st();
+                    if (!wide) join_copies(top, lt);
                 }
-                if (pos + TC_BLOCK > x.s.len && !clear_tail(j, pos)) break;
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[w]);
             }
             ring0 += 2 * n;
-
-            // ---- the segment's result
-            float m1 = -INFINITY, l1 = 0.f;
-            if (!wide && n > 0) {
-                if (w == 1) { sh.ml[r][0] = m; sh.ml[r][1] = l; }
-                softmax_bar_or(false);
-                if (w == 0) { m1 = sh.ml[r][0]; l1 = sh.ml[r][1]; }
-            }
-            if (w == 0 || wide) {
-                if (n > 0) {
-                    wait(&sh.o_full[w], ph_o[w], 7);
-                    ph_o[w] ^= 1;
-                }
-                if (w == 0 && (wide ? n > 0 : n > 1)) {
-                    if (!wide) wait(&sh.o_full[1], ph_o[1], 8);
-                    ph_o[1] ^= 1;
-                }
-                tc_fence_after();
-                const bool two = !wide && n > 1;
-                const float top = fmaxf(m, m1);
-                const float b0 = m == -INFINITY ? 0.f : ex2(m - top), b1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
-                const float lt = l * b0 + l1 * b1;
-                const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
-                float size = 0.f;
-                const int wr = wide ? w * 128 + r : r;
-                const bool part = mine && !whole;
-                if (warp_mine && ok) {
-                    uint16_t *out = (uint16_t *)a.out + row * a.os[0] + head * a.os[1];
-                    float *pt = p.part + ((long long)slot * p.ws_rows + wr) * D;
-#pragma unroll
-                    for (int h = 0; h < D; h += 32) {
-                        uint32_t o[32];
-                        float *f = (float *)o;
-                        if (n > 0) {
-                            tm_ld32(to + h, o);
-                            tm_wait_ld();
-                            pin32(o);
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = 0;
-                        }
-                        // (a group whose maximum is still -inf has weights of 0 only, and its O holds zeros)
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) f[k] *= b0;
-                        if (two) {
-                            uint32_t o1[32];
-                            tm_ld32(to + D + h, o1);
-                            tm_wait_ld();
-                            pin32(o1);
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) f[k] = fmaf(__uint_as_float(o1[k]), b1, f[k]);
-                        }
-                        if (part) {
-#pragma unroll
-                            for (int k = 0; k < 32; k += 4) *(float4 *)(pt + h + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
-                        } else if (mine) {
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) { f[k] *= inv; size += fabsf(f[k]); }
-#pragma unroll
-                            for (int k = 0; k < 32; k += 8)
-                                *(uint4 *)(out + h + k) = make_uint4(pack16<BF>(f[k], f[k + 1]), pack16<BF>(f[k + 2], f[k + 3]),
-                                                                     pack16<BF>(f[k + 4], f[k + 5]), pack16<BF>(f[k + 6], f[k + 7]));
-                        }
-                    }
-                    if (part) *(float2 *)(p.ml + ((long long)slot * p.ws_rows + wr) * 2) = make_float2(top, lt);
-                    if (mine && whole && !(size < INFINITY)) sh.odd = 1;   // (see attend_join_kernel)
-                }
-            } else if (n > 1) {
-                ph_o[1] ^= 1;
-            }
-            }
-            // the first of a cut tile's pieces says how many follow
-            if (!whole && wk.j0 == 0) {
-                meta = true;
-                if (tid == 0) {
-                    const int first = x.base + TC_OVERHEAD + 2, last = x.base + TC_OVERHEAD + x.nb - 2;   // cuts that stay inside the tile
-                    int *mt = p.meta + cta * 8;
-                    mt[0] = last / per - (first - 1) / per;
-                    mt[1] = x.seq; mt[2] = x.tok0; mt[3] = x.ntok; mt[4] = x.h; mt[5] = wide;
-                }
-            }
             tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.seg_empty[n_seg % TC_SEGS]);
+            ++n_seg;
+            if (!ok) break;
         }
-        if (!meta && tid == 0) p.meta[cta * 8] = 0;
     }
 
     // ---- close: no copy and no tensor instruction may be in flight when the CTA ends
@@ -866,32 +1037,33 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
 // An infinity or NaN in V at a position that some rows of a tile do not see has met their weight of 0 in the product.  Such
 // rows show it by not being finite; they are done over here, position by position.
 template <int D, int TY>
-__global__ void __launch_bounds__(512) attend_join_kernel(const __grid_constant__ TcParams p) {
+__global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ TcParams p) {
     constexpr int E = D / 32;
     typedef typename Elem<TY>::T T;
     typedef typename Elem<TY == PTY_BF16 ? PTY_BF16 : PTY_F16>::T C;
     const AttendParams &a = p.a;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
     const int *mt = p.meta + blockIdx.x * 8;
-    const int more = mt[0];
+    const int more = mt[0], row0 = mt[1], ntok = mt[2], h = mt[3], wide = mt[4];
     int odd = 0;
     for (int i = threadIdx.x; i < p.n_ctas; i += blockDim.x) odd |= p.meta[i * 8 + 6];
+    auto over = [&](int t, int hd) {
+        const int i = batch_find(a.B, t);
+        if (i >= 0) attend_row<D, T, C>(a, batch_seq(a.P, a.B, i), t, hd, lane);
+    };
     if (__syncthreads_or(odd)) {
-        for (long long u = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * 16 + (threadIdx.x >> 5); u < (long long)a.B.rows * a.heads;
-             u += (long long)gridDim.x * gridDim.y * 16) {
-            const int t = (int)(u / a.heads), hd = (int)(u % a.heads), i = batch_find(a.B, t);
-            if (i < 0) continue;
-            const T *o = (const T *)a.out + t * a.os[0] + hd * a.os[1] + (threadIdx.x & 31) * E;
-            float size = 0.f;
-            for (int e = 0; e < E; ++e) size += fabsf(to_f32(o[e]));
-            if (__any_sync(~0u, !(size < INFINITY))) attend_row<D, T, C>(a, batch_seq(a.P, a.B, i), t, hd, threadIdx.x & 31);
-        }
+        for (int t = blockIdx.y * gridDim.x + blockIdx.x; t < a.B.rows; t += gridDim.x * gridDim.y)
+            for (int hd = warp; hd < a.heads; hd += 8) {
+                const T *o = (const T *)a.out + t * a.os[0] + hd * a.os[1] + lane * E;
+                float size = 0.f;
+                for (int e = 0; e < E; ++e) size += fabsf(to_f32(o[e]));
+                if (__any_sync(~0u, !(size < INFINITY))) over(t, hd);
+            }
     }
     if (more <= 0 || more >= p.n_ctas - (int)blockIdx.x) return;
-    const int seq = mt[1], tok0 = mt[2], ntok = mt[3], h = mt[4], wide = mt[5];
-    const SeqRows s = batch_seq(a.P, a.B, seq);
-    const int tq = 128 / a.group, lane = threadIdx.x & 31;
-    const int n_rows = wide ? 256 : ntok * a.group;
-    for (int r = blockIdx.y * 16 + (threadIdx.x >> 5); r < n_rows; r += 16 * gridDim.y) {
+    const int tq = 128 / a.group, n_rows = wide ? 128 + (ntok - tq) * a.group : ntok * a.group;
+    for (int r = blockIdx.y * 8 + warp; r < n_rows; r += 8 * gridDim.y) {
         const int half = r >> 7, rr = r & 127, tok = (wide ? half * tq : 0) + rr / a.group;
         if (rr >= tq * a.group || tok >= ntok) continue;
         auto at = [&](int piece) { return (long long)(piece ? 2 * ((int)blockIdx.x + piece) : 2 * (int)blockIdx.x + 1) * p.ws_rows + r; };
@@ -899,23 +1071,34 @@ __global__ void __launch_bounds__(512) attend_join_kernel(const __grid_constant_
         for (int i = lane; i <= more; i += 32) top = fmaxf(top, p.ml[at(i) * 2]);
         for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
         for (int e = 0; e < E; ++e) o[e] = 0.f;
-        for (int i = 0; i <= more; ++i) {
-            const float2 ml = *(const float2 *)(p.ml + at(i) * 2);
-            if (ml.x == -INFINITY) continue;
-            const float b = ex2(ml.x - top);
-            l += b * ml.y;
-            const float *src = p.part + at(i) * D + lane * E;
-            for (int e = 0; e < E; ++e) o[e] = fmaf(b, src[e], o[e]);
+        for (int i0 = 0; i0 <= more; i0 += 32) {
+            float b = 0.f, lb = 0.f;   // lane i: the weight of piece i0 + i
+            if (i0 + lane <= more) {
+                const float2 ml = *(const float2 *)(p.ml + at(i0 + lane) * 2);
+                if (ml.x != -INFINITY) { b = ex2(ml.x - top); lb = b * ml.y; }
+            }
+            l += lb;
+            const int n = min(32, more + 1 - i0);
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+                const float bi = __shfl_sync(~0u, b, i);
+                const float *src = p.part + at(i0 + i) * D + lane * E;
+                float v[E];
+                if constexpr (E == 4) *(float4 *)v = *(const float4 *)src;
+                else *(float2 *)v = *(const float2 *)src;
+                for (int e = 0; e < E; ++e) o[e] = fmaf(bi, v[e], o[e]);
+            }
         }
+        for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(~0u, l, x);
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
         float size = 0.f;
         for (int e = 0; e < E; ++e) { o[e] *= inv; size += fabsf(o[e]); }
-        const int row = s.first + tok0 + tok, head = h * a.group + rr % a.group;
+        const int row = row0 + tok, head = h * a.group + rr % a.group;
         T *out = (T *)a.out + row * a.os[0] + head * a.os[1] + lane * E;
         for (int e = 0; e < E; ++e) from_f32(out + e, o[e]);
         if (__any_sync(~0u, !(size < INFINITY))) {
             __syncwarp();
-            attend_row<D, T, C>(a, s, row, head, lane);
+            over(row, head);
         }
     }
 }
@@ -950,7 +1133,7 @@ bool page_map(CUtensorMap *m, const PagesDev &P, const uint16_t *base, const lon
 struct TcSize { size_t meta, ml, part; int rows; };
 TcSize tc_size(const AttendParams &p, int n_sm) {
     TcSize s;
-    const TcGeom g = tc_geom(p);
+    const TcBatch g(p, nullptr);
     s.rows = p.B.rows > g.tq ? (g.step > g.tq ? 256 : 128) : p.B.rows * p.group;
     s.meta = ((size_t)n_sm * 8 * 4 + 255) / 256 * 256;
     s.ml = ((size_t)n_sm * 2 * s.rows * 2 * 4 + 255) / 256 * 256;
@@ -979,7 +1162,17 @@ cudaError_t launch_tc(const AttendParams &p, int n_sm, void *ws, long long wait_
     attend_tc_kernel<D, TY><<<n_sm, TC_THREADS, smem, st>>>(q, km, vm);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    attend_join_kernel<D, TY><<<dim3(n_sm, z.rows == 256 ? 4 : 1), 512, 0, st>>>(q);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n_sm, (z.rows + 31) / 32);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, attend_join_kernel<D, TY>, q);
+    if (e != cudaSuccess) return e;
     *launches += 2;
     return cudaGetLastError();
 }

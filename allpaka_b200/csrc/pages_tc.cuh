@@ -58,6 +58,10 @@ __device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t *r) {
                  APK_I8(r, 0), APK_I8(r, 8), APK_I8(r, 16), APK_I8(r, 24)
                  : "memory");
 }
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), APK_I8(r, 0), APK_I8(r, 8)
+                 : "memory");
+}
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
