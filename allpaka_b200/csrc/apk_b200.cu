@@ -8,6 +8,7 @@
 #include "../../include/allpaka_b200.h"
 #include "kernels.cuh"
 #include "mv_pick.h"
+#include "pages.cuh"
 
 #include <dlfcn.h>
 
@@ -873,6 +874,7 @@ int apk_init(apk_ctx **out, int device) {
     // starts before the launch in front of it has drained
     APK_TRY(c->partials.ensure(2 * (size_t)c->n_sm * 2 * MAX_M_EFF * TILE_ROWS * sizeof(unsigned long long), true));
     APK_TRY(init_kernel_attrs(c.get()));
+    CUDA_TRY(prepare_attend());
     if (const char *e = getenv("ALLPAKA_B200_PDL")) c->use_pdl = atoi(e) != 0;
     if (const char *e = getenv("ALLPAKA_B200_FUSE_NORM")) c->fuse_norm = atoi(e);
     if (const char *e = getenv("ALLPAKA_B200_INFLIGHT")) c->inflight = std::max(1, std::min(atoi(e), MAX_STAGES));

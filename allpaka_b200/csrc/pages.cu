@@ -27,26 +27,188 @@ __device__ __forceinline__ void put(void *p, long long i, int ty, float x) {
 
 // ---------------------------------------------------------------------------------------------- rope_append
 
-// One block per row of the batch.  Angles: position * turns(pair) in 64 bits, whole turns taken off, then sine and
-// cosine of the rest in 32 bits: at a position of 2^20 a 32-bit product would already be 2^-4 radians off.
+// Where a row of the batch belongs: its position in its sequence and where that is stored (-1: nowhere; -2: the row is nobody's).
+struct RopeAt { int pos, page; };
+constexpr int ROPE_MOST = 8;   // rows that a block takes
+
+// The places and the sines and cosines of a block's rows, side by side: a warp looks for a row's sequence, 32 offsets at a time
+// instead of a chain of loads.  Angles: position * turns(pair) in 64 bits, whole turns taken off, then sine and cosine of the rest
+// in 32 bits: at a position of 2^20 a 32-bit product would already be 2^-4 radians off.
+__device__ __forceinline__ void rope_places(const RopeParams &p, int t0, int rows, RopeAt *at, int *turn_at, float2 *cs) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp < rows) {
+        const int t = t0 + warp;
+        int before = 0;   // sequences that begin at row t or before
+        for (int i0 = 0; i0 < p.B.n; i0 += 32) before += __popc(__ballot_sync(~0u, i0 + lane < p.B.n && p.B.cu[i0 + lane] <= t));
+        RopeAt r = {0, -2};
+        int rp = 0;
+        if (before > 0 && t < p.B.cu[before]) {
+            const SeqRows s = batch_seq(p.P, p.B, before - 1);
+            r.pos = s.len - s.rows + (t - s.first);
+            rp = p.positions ? p.positions[t] : r.pos;
+            r.page = r.pos >= 0 && r.pos < s.len ? page_of(p.P, s.slot, r.pos) : -1;
+        }
+        if (lane == 0) { at[warp] = r; turn_at[warp] = rp; }
+    }
+    __syncthreads();
+    const int half = p.rot / 2;
+    for (int i = threadIdx.x; i < rows * half; i += 256) {
+        const int row = i / half, j = i - row * half;
+        const double a = (double)turn_at[row] * p.turn[j];
+        float sn, cn;
+        sincospif((float)(2.0 * (a - rint(a))), &sn, &cn);
+        cs[row * 128 + j] = make_float2(cn * p.mag, sn * p.mag);
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ void rope_turn(float &a, float &b, float2 z) {
+    const float x = a * z.x - b * z.y, y = b * z.x + a * z.y;
+    a = x;
+    b = y;
+}
+
+// Sixteen values of a row at two offsets, as they are stored, and as 32-bit values.
+template <int TY> struct Raw16 { uint4 v[TY == PTY_F32 ? 4 : 2]; };
+template <int TY>
+__device__ __forceinline__ void load16(Raw16<TY> &x, const typename Elem<TY>::T *src, int o0, int o1) {
+    if constexpr (TY == PTY_F32) {
+        x.v[0] = __ldcs((const uint4 *)(src + o0)); x.v[1] = __ldcs((const uint4 *)(src + o0 + 4));
+        x.v[2] = __ldcs((const uint4 *)(src + o1)); x.v[3] = __ldcs((const uint4 *)(src + o1 + 4));
+    } else {
+        x.v[0] = __ldcs((const uint4 *)(src + o0));
+        x.v[1] = __ldcs((const uint4 *)(src + o1));
+    }
+}
+template <int TY>
+__device__ __forceinline__ void widen16(const Raw16<TY> &x, float *y) {
+#pragma unroll
+    for (int h = 0; h < (TY == PTY_F32 ? 4 : 2); ++h) {
+        const uint32_t u[4] = {x.v[h].x, x.v[h].y, x.v[h].z, x.v[h].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (TY == PTY_F32) {
+                y[4 * h + e] = __uint_as_float(u[e]);
+            } else {
+                float2 f;
+                if constexpr (TY == PTY_F16) f = __half22float2(*(const __half2 *)&u[e]);
+                else f = __bfloat1622float2(*(const __nv_bfloat162 *)&u[e]);
+                y[8 * h + 2 * e] = f.x;
+                y[8 * h + 2 * e + 1] = f.y;
+            }
+        }
+    }
+}
+__device__ __forceinline__ void store8(void *p, long long at, int ty, const float *x) {
+    if (ty == PTY_F32) {
+        *(float4 *)((float *)p + at) = *(const float4 *)x;
+        *(float4 *)((float *)p + at + 4) = *(const float4 *)(x + 4);
+        return;
+    }
+    uint32_t u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (ty == PTY_F16) { const __half2 h = __floats2half2_rn(x[2 * e], x[2 * e + 1]); u[e] = *(const uint32_t *)&h; }
+        else { const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]); u[e] = *(const uint32_t *)&h; }
+    }
+    *(uint4 *)((uint16_t *)p + at) = make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// Heads of 16 * LANES dimensions, rotated in whole groups of 16: LANES threads a head, 16 values each (8 pairs, or 16 that pass
+// through), so that every access is 16 bytes wide.  Bound by the bytes; what stands in the way is latency: finding a row's place
+// and its angles is a chain of four loads and 64-bit arithmetic, about 2 us, so a block of a long batch takes eight rows, works
+// their places out together, and has its first loads under way before it begins.
+template <int TY, int LANES>
+__global__ void __launch_bounds__(256) rope_append_wide_kernel(const __grid_constant__ RopeParams p) {
+    typedef typename Elem<TY>::T T;
+    constexpr int AHEAD = TY == PTY_F32 ? 2 : 4, AT_ONCE = 256 / LANES;   // heads that the block works on side by side
+    __shared__ float2 cs[ROPE_MOST * 128];
+    __shared__ RopeAt place[ROPE_MOST];
+    __shared__ int turn_at[ROPE_MOST];
+    pages_let_next();
+    pages_wait_front();
+    const int t0 = blockIdx.x * p.rows_per_block, rows = min(p.rows_per_block, p.B.rows - t0);
+    const int u = threadIdx.x % LANES, heads = p.heads + 2 * p.P.kv, units = rows * heads;
+    const bool turned = u < p.rot / 16;
+    const int o0 = turned && !p.pairs ? u * 8 : u * 16, o1 = turned && !p.pairs ? p.rot / 2 + u * 8 : u * 16 + 8;
+    Raw16<TY> raw[AHEAD];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            const int i = i0 + a * AT_ONCE + threadIdx.x / LANES;
+            if (i >= units) break;
+            const int t = t0 + i / heads, r = i % heads;
+            const T *src = r < p.heads ? (const T *)p.q + t * p.qs[0] + r * p.qs[1]
+                           : r < p.heads + p.P.kv ? (const T *)p.k + t * p.ks[0] + (r - p.heads) * p.ks[1]
+                                                  : (const T *)p.v + t * p.vs[0] + (r - p.heads - p.P.kv) * p.vs[1];
+            load16<TY>(raw[a], src, o0, o1);
+        }
+    };
+    load(0);
+    rope_places(p, t0, rows, place, turn_at, cs);
+    const int cache = p.P.bf16 ? PTY_BF16 : PTY_F16;
+    for (int i0 = 0; i0 < units; i0 += AHEAD * AT_ONCE) {
+        if (i0) load(i0);
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (i0 + a * AT_ONCE >= units) break;   // (the whole block)
+            const int i = i0 + a * AT_ONCE + threadIdx.x / LANES, row = min(i / heads, rows - 1), r = i % heads;
+            float y[16];
+            widen16<TY>(raw[a], y);
+            const int kind = r < p.heads ? 0 : (r < p.heads + p.P.kv ? 1 : 2);
+            if (p.q_norm || p.k_norm) {
+                const float *w = kind == 0 ? p.q_norm : (kind == 1 ? p.k_norm : nullptr);
+                float ss = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) ss = fmaf(y[e], y[e], ss);
+#pragma unroll
+                for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+                if (w) {
+                    const float rs = rsqrtf(ss / (float)p.P.dim + p.eps);
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const float4 g = __ldg((const float4 *)(w + (e < 8 ? o0 + e : o1 + e - 8)));
+                        y[e] *= rs * g.x; y[e + 1] *= rs * g.y; y[e + 2] *= rs * g.z; y[e + 3] *= rs * g.w;
+                    }
+                }
+            }
+            if (kind < 2 && turned) {
+                const float2 *z = cs + row * 128 + u * 8;
+                if (p.pairs) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) rope_turn(y[2 * e], y[2 * e + 1], z[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) rope_turn(y[e], y[8 + e], z[e]);
+                }
+            }
+            const RopeAt at = place[row];
+            if (i >= units || at.page == -2 || (kind && at.page < 0)) continue;
+            const long long t = t0 + row, in = at.pos & (p.P.page - 1);
+            void *dst = p.out;
+            long long to = t * p.os[0] + r * p.os[1];
+            if (kind == 1) { dst = p.P.k; to = p.layer * p.P.ks[0] + at.page * p.P.ks[1] + in * p.P.ks[2] + (r - p.heads) * p.P.ks[3]; }
+            if (kind == 2) { dst = p.P.v; to = p.layer * p.P.vs[0] + at.page * p.P.vs[1] + in * p.P.vs[2] + (r - p.heads - p.P.kv) * p.P.vs[3]; }
+            const int ty = kind ? cache : p.out_ty;
+            store8(dst, to + o0, ty, y);
+            store8(dst, to + o1, ty, y + 8);
+        }
+    }
+}
+
+// Any other head: a warp per head, value by value.
 template <int TY>
 __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant__ RopeParams p) {
     typedef typename Elem<TY>::T T;
     __shared__ float2 cs[128];
+    __shared__ RopeAt place;
+    __shared__ int turn_at;
+    pages_let_next();
+    pages_wait_front();
     const int t = blockIdx.x;
-    const int i = batch_find(p.B, t);
-    if (i < 0) return;
-    const SeqRows s = batch_seq(p.P, p.B, i);
-    const int pos = s.len - s.rows + (t - s.first);
-    const int rp = p.positions ? p.positions[t] : pos;
-    for (int j = threadIdx.x; j < p.rot / 2; j += blockDim.x) {
-        const double a = (double)rp * p.turn[j];
-        float sn, cn;
-        sincospif((float)(2.0 * (a - rint(a))), &sn, &cn);
-        cs[j] = make_float2(cn * p.mag, sn * p.mag);
-    }
-    __syncthreads();
-    const int page = pos >= 0 && pos < s.len ? page_of(p.P, s.slot, pos) : -1;
+    rope_places(p, t, 1, &place, &turn_at, cs);
+    const int pos = place.pos, page = place.page;
+    if (page == -2) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.P.dim;
     const int n_rows = p.heads + 2 * p.P.kv;
     for (int r = warp; r < n_rows; r += 8) {
@@ -115,6 +277,8 @@ __device__ __forceinline__ void drop_pages(const PagesDev &P, int slot, int from
 // dst takes over src's pages and length in place of what it held: one block per pair.  The host has checked that no
 // slot is named twice as a destination and none is a source too.
 __global__ void __launch_bounds__(256) pages_fork_kernel(const __grid_constant__ PagesDev P, const __grid_constant__ SlotList l) {
+    pages_let_next();
+    pages_wait_front();
     const int src = l.a[blockIdx.x], dst = l.b[blockIdx.x];
     const int len = pages_len(P, src), n = pages_for(P, len);
     drop_pages(P, dst, 0, pages_for(P, pages_len(P, dst)));
@@ -131,6 +295,8 @@ __global__ void __launch_bounds__(256) pages_fork_kernel(const __grid_constant__
 
 // The sequence keeps its first b positions; the pages behind them lose a holder.
 __global__ void __launch_bounds__(256) pages_release_kernel(const __grid_constant__ PagesDev P, const __grid_constant__ SlotList l) {
+    pages_let_next();
+    pages_wait_front();
     const int slot = l.a[blockIdx.x];
     const int len = pages_len(P, slot), keep = min(len, l.b[blockIdx.x]);
     drop_pages(P, slot, pages_for(P, keep), pages_for(P, len));
@@ -168,6 +334,8 @@ __global__ void __launch_bounds__(PAGES_MAX_LIST) pages_reserve_kernel(const __g
     const int i = threadIdx.x;
     int *const list = P.work + PW_LIST;
     int *const fresh = list + 4 * P.n_seqs;
+    pages_let_next();
+    pages_wait_front();
     if (i == 0) n_copies = too_long = 0;
     int slot = 0, old = 0, have = 0, want = 0, last = -1;
     if (i < l.n) {
@@ -232,25 +400,49 @@ __global__ void __launch_bounds__(PAGES_MAX_LIST) pages_reserve_kernel(const __g
     if (i == 0) { P.work[PW_SHORT] = 0; P.work[PW_COPIES] = n_copies; }
 }
 
-// The copy list, in every layer, K and V: 16 bytes a thread and turn.
-__device__ __forceinline__ void copy_pages(const PagesDev &P, const int *list, int n, int block, int blocks) {
-    const int vecs = P.dim / 8;
-    for (int u = block; u < n * P.n_layers * 2; u += blocks) {
-        const int e = u / (P.n_layers * 2), lk = u % (P.n_layers * 2), layer = lk >> 1;
-        const int src = list[4 * e], dst = list[4 * e + 1], tok = list[4 * e + 2];
+// Copies of pages' positions in every layer, K and V.  A piece is 1024 16-byte vectors, four a thread, all asked for before the
+// first is stored; pieces are dealt out over all blocks.  copy(e, src, dst, positions): what entry e is.
+template <typename Copy>
+__device__ __forceinline__ void copy_pages(const PagesDev &P, int n, const Copy &copy) {
+    const int vecs = P.dim / 8, per_pos = P.kv * vecs, pieces = (P.page * per_pos + 1023) / 1024;
+    const bool flat = P.ks[3] == P.dim && P.vs[3] == P.dim && P.ks[2] == (long long)P.kv * P.dim && P.vs[2] == (long long)P.kv * P.dim;
+    for (long long u = blockIdx.x; u < (long long)n * P.n_layers * 2 * pieces; u += gridDim.x) {
+        const int piece = (int)(u % pieces), lk = (int)(u / pieces) % (2 * P.n_layers), e = (int)(u / pieces) / (2 * P.n_layers);
+        int src, dst, positions;
+        copy(e, src, dst, positions);
+        const int total = positions * per_pos;
         const long long *st = lk & 1 ? P.vs : P.ks;
-        uint16_t *base = (lk & 1 ? P.v : P.k) + layer * st[0];
-        const int total = tok * P.kv * vecs;
-        for (int x = threadIdx.x; x < total; x += blockDim.x) {
-            const int d = x % vecs, y = x / vecs, h = y % P.kv, t = y / P.kv;
-            const long long off = t * st[2] + h * st[3] + d * 8;
-            *(uint4 *)(base + dst * st[1] + off) = *(const uint4 *)(base + src * st[1] + off);
+        uint16_t *base = (lk & 1 ? P.v : P.k) + (lk >> 1) * st[0];
+        const uint16_t *from = base + src * st[1];
+        uint16_t *to = base + dst * st[1];
+        uint4 v[4];
+        long long off[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int x = piece * 1024 + i * 256 + threadIdx.x;
+            if (flat) {
+                off[i] = (long long)x * 8;
+            } else {
+                const int d = x % vecs, y = x / vecs;
+                off[i] = (y / P.kv) * st[2] + (y % P.kv) * st[3] + d * 8;
+            }
+            if (x < total) v[i] = __ldcs((const uint4 *)(from + off[i]));
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (piece * 1024 + i * 256 + threadIdx.x < total) __stcs((uint4 *)(to + off[i]), v[i]);
     }
 }
 
 __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__ PagesDev P) {
-    copy_pages(P, P.work + PW_LIST, min(P.work[PW_COPIES], P.n_seqs), blockIdx.x, gridDim.x);
+    pages_let_next();
+    pages_wait_front();
+    const int *list = P.work + PW_LIST;
+    copy_pages(P, min(P.work[PW_COPIES], P.n_seqs), [&](int e, int &src, int &dst, int &positions) {
+        src = list[4 * e];
+        dst = list[4 * e + 1];
+        positions = list[4 * e + 2];
+    });
 }
 
 // Where every page goes: live pages whose number is not below the number of live pages move into the free pages
@@ -258,6 +450,8 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__
 __global__ void __launch_bounds__(1024) pages_plan_kernel(const __grid_constant__ PagesDev P, int *map) {
     __shared__ int sh[32];
     const int i = threadIdx.x;
+    pages_let_next();
+    pages_wait_front();
     int live = 0;
     for (int pg = i; pg < P.n_pages; pg += 1024) live += P.refs[pg] > 0;
     block_scan(live, sh);
@@ -287,6 +481,8 @@ __global__ void __launch_bounds__(1024) pages_plan_kernel(const __grid_constant_
 }
 
 __global__ void __launch_bounds__(256) pages_move_kernel(const __grid_constant__ PagesDev P, const int *map) {
+    pages_let_next();
+    pages_wait_front();
     const int *holes = P.work + PW_LIST + 4 * P.n_seqs, *movers = holes + P.n_pages;
     for (int s = blockIdx.x; s < P.n_seqs; s += gridDim.x) {
         int *row = P.table + (long long)s * P.table_stride;
@@ -296,59 +492,67 @@ __global__ void __launch_bounds__(256) pages_move_kernel(const __grid_constant__
             if ((unsigned)pg < (unsigned)P.n_pages && map[pg] >= 0) row[c] = map[pg];
         }
     }
-    const int n = P.work[PW_COPIES], vecs = P.dim / 8;
-    for (int u = blockIdx.x; u < n * P.n_layers * 2; u += gridDim.x) {
-        const int e = u / (P.n_layers * 2), lk = u % (P.n_layers * 2), layer = lk >> 1;
-        const int src = movers[e], dst = holes[e];
-        const long long *st = lk & 1 ? P.vs : P.ks;
-        uint16_t *base = (lk & 1 ? P.v : P.k) + layer * st[0];
-        const int total = P.page * P.kv * vecs;
-        for (int x = threadIdx.x; x < total; x += blockDim.x) {
-            const int d = x % vecs, y = x / vecs, h = y % P.kv, t = y / P.kv;
-            const long long off = t * st[2] + h * st[3] + d * 8;
-            *(uint4 *)(base + dst * st[1] + off) = *(const uint4 *)(base + src * st[1] + off);
-        }
-    }
+    copy_pages(P, P.work[PW_COPIES], [&](int e, int &src, int &dst, int &positions) {
+        src = movers[e];
+        dst = holes[e];
+        positions = P.page;
+    });
+}
+
+// Blocks for n copies: eight a multiprocessor at most, each with something to do.
+unsigned copy_blocks(const PagesDev &P, long long n, int n_sm) {
+    const long long pieces = (P.page * P.kv * (P.dim / 8) + 1023) / 1024;
+    return (unsigned)std::max<long long>(1, std::min<long long>(8 * n_sm, n * P.n_layers * 2 * pieces));
 }
 
 }  // namespace
 
-cudaError_t launch_rope_append(const RopeParams &p, int, cudaStream_t st, int *launches) {
-    if (p.ty == PTY_F32) rope_append_kernel<PTY_F32><<<p.B.rows, 256, 0, st>>>(p);
-    else if (p.ty == PTY_F16) rope_append_kernel<PTY_F16><<<p.B.rows, 256, 0, st>>>(p);
-    else rope_append_kernel<PTY_BF16><<<p.B.rows, 256, 0, st>>>(p);
+template <int TY>
+cudaError_t launch_rope(RopeParams p, int n_sm, cudaStream_t st) {
+    // weights are read 16 bytes at a time; their start is the caller's
+    const bool weights = (((uintptr_t)p.q_norm | (uintptr_t)p.k_norm) & 15) == 0;
+    if (p.rot % 16 == 0 && weights && (p.P.dim == 64 || p.P.dim == 128 || p.P.dim == 256)) {
+        // one row a block while that fills the multiprocessors twice over, up to eight as the batch grows
+        p.rows_per_block = std::max(1, std::min(ROPE_MOST, p.B.rows / (2 * n_sm)));
+        const dim3 grid((p.B.rows + p.rows_per_block - 1) / p.rows_per_block);
+        if (p.P.dim == 64) return launch_front(rope_append_wide_kernel<TY, 4>, grid, 256, 0, st, p);
+        if (p.P.dim == 128) return launch_front(rope_append_wide_kernel<TY, 8>, grid, 256, 0, st, p);
+        return launch_front(rope_append_wide_kernel<TY, 16>, grid, 256, 0, st, p);
+    }
+    return launch_front(rope_append_kernel<TY>, dim3(p.B.rows), 256, 0, st, p);
+}
+
+cudaError_t launch_rope_append(const RopeParams &p, int n_sm, cudaStream_t st, int *launches) {
     *launches += 1;
-    return cudaGetLastError();
+    if (p.ty == PTY_F32) return launch_rope<PTY_F32>(p, n_sm, st);
+    if (p.ty == PTY_F16) return launch_rope<PTY_F16>(p, n_sm, st);
+    return launch_rope<PTY_BF16>(p, n_sm, st);
 }
 
 cudaError_t launch_pages_fork(const PagesDev &P, const SlotList &l, cudaStream_t st, int *launches) {
-    pages_fork_kernel<<<l.n, 256, 0, st>>>(P, l);
     *launches += 1;
-    return cudaGetLastError();
+    return launch_front(pages_fork_kernel, dim3(l.n), 256, 0, st, P, l);
 }
 
 cudaError_t launch_pages_release(const PagesDev &P, const SlotList &l, cudaStream_t st, int *launches) {
-    pages_release_kernel<<<l.n, 256, 0, st>>>(P, l);
     *launches += 1;
-    return cudaGetLastError();
+    return launch_front(pages_release_kernel, dim3(l.n), 256, 0, st, P, l);
 }
 
 cudaError_t launch_pages_reserve(const PagesDev &P, const SlotList &l, int n_sm, cudaStream_t st, int *launches) {
-    pages_reserve_kernel<<<1, PAGES_MAX_LIST, 0, st>>>(P, l);
     *launches += 1;
-    if (l.n) {
-        pages_copy_kernel<<<(unsigned)std::min<long long>(4 * n_sm, (long long)l.n * P.n_layers * 2), 256, 0, st>>>(P);
-        *launches += 1;
-    }
-    return cudaGetLastError();
+    cudaError_t e = launch_front(pages_reserve_kernel, dim3(1), PAGES_MAX_LIST, 0, st, P, l);
+    if (e != cudaSuccess || l.n == 0) return e;
+    *launches += 1;
+    return launch_front(pages_copy_kernel, dim3(copy_blocks(P, l.n, n_sm)), 256, 0, st, P);
 }
 
 cudaError_t launch_pages_compact(const PagesDev &P, int *page_map, int n_sm, cudaStream_t st, int *launches) {
     if (!page_map) page_map = P.work + PW_LIST + 4 * P.n_seqs + 2 * P.n_pages;
-    pages_plan_kernel<<<1, 1024, 0, st>>>(P, page_map);
-    pages_move_kernel<<<4 * n_sm, 256, 0, st>>>(P, page_map);
     *launches += 2;
-    return cudaGetLastError();
+    cudaError_t e = launch_front(pages_plan_kernel, dim3(1), 1024, 0, st, P, page_map);
+    if (e != cudaSuccess) return e;
+    return launch_front(pages_move_kernel, dim3(copy_blocks(P, P.n_pages / 2 + 1, n_sm)), 256, 0, st, P, (const int *)page_map);
 }
 
 }  // namespace apk

@@ -106,10 +106,30 @@ struct RopeParams {
     const int *positions;        // per row, or null: the row's own position in its sequence
     const float *q_norm, *k_norm;
     float eps;
+    int rows_per_block;          // (the launch's)
     int rot, pairs;              // dimensions rotated; 1: neighbouring pairs, 0: halves
     float mag;                   // factor on sine and cosine
     double turn[128];            // turns a position, per pair
 };
+
+// Programmatic dependent launch: the kernel may be placed while the one in front of it in the stream is still ending.  Every
+// kernel that is launched so calls pages_wait_front() before it reads or writes anything that another one touches.
+template <typename... Args>
+cudaError_t launch_front(void (*kernel)(Args...), dim3 grid, int block, size_t smem, cudaStream_t st, const Args &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+__device__ __forceinline__ void pages_wait_front() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pages_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 struct SlotList {
     int n;
@@ -117,6 +137,7 @@ struct SlotList {
 };
 
 cudaError_t launch_rope_append(const RopeParams &p, int n_sm, cudaStream_t st, int *launches);
+cudaError_t prepare_attend();   // once per context, on its device
 size_t attend_ws_bytes(const AttendParams &p, int n_sm);
 cudaError_t launch_attend(const AttendParams &p, int n_sm, void *ws, long long wait_limit, cudaStream_t st, int *launches);
 cudaError_t launch_pages_fork(const PagesDev &P, const SlotList &l, cudaStream_t st, int *launches);

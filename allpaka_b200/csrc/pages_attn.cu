@@ -508,7 +508,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int tq = 128 / a.group;
 
-    pdl_launch_dependents();   // (attend_join_kernel waits for this grid's end)
+    pages_let_next();   // (attend_join_kernel waits for this grid's end)
     if (tid == 0) {
         for (int i = 0; i < TC_STAGES; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
         for (int i = 0; i < TC_SEGS; ++i) { mbar_init(&sh.seg_full[i], 1); mbar_init(&sh.seg_empty[i], 10); }
@@ -522,6 +522,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
         fence_mbar_init();
     }
     if (warp == 9) tm_alloc(&sh.tmem, 512);
+    pages_wait_front();
     for (int i = tid; i < min(a.B.n, TC_INFO); i += TC_THREADS) sh.info[i] = batch_seq(a.P, a.B, i);
     tc_fence_before();
     __syncthreads();
@@ -1043,7 +1044,8 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     typedef typename Elem<TY == PTY_BF16 ? PTY_BF16 : PTY_F16>::T C;
     const AttendParams &a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    pdl_wait();
+    pages_let_next();
+    pages_wait_front();
     const int *mt = p.meta + blockIdx.x * 8;
     const int more = mt[0], row0 = mt[1], ntok = mt[2], h = mt[3], wide = mt[4];
     int odd = 0;
@@ -1141,10 +1143,19 @@ TcSize tc_size(const AttendParams &p, int n_sm) {
     return s;
 }
 
+template <int D>
+constexpr int tc_smem() {
+    constexpr int n = 1024 + (2 + TC_STAGES) * TC_BLOCK * D * 2 + (int)sizeof(TcShared) + 4 * PAGES_MAX_BATCH;
+    static_assert(n <= 232448, "shared memory of a block");
+    return n;
+}
+
+template <int D, int TY>
+cudaError_t tc_prepare() { return cudaFuncSetAttribute(attend_tc_kernel<D, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, tc_smem<D>()); }
+
 template <int D, int TY>
 cudaError_t launch_tc(const AttendParams &p, int n_sm, void *ws, long long wait_limit, cudaStream_t st, int *launches) {
-    constexpr int smem = 1024 + (2 + TC_STAGES) * TC_BLOCK * D * 2 + (int)sizeof(TcShared) + 4 * PAGES_MAX_BATCH;
-    static_assert(smem <= 232448, "shared memory of a block");
+    constexpr int smem = tc_smem<D>();
     CUtensorMap km, vm;
     if (!page_map(&km, p.P, p.P.k + p.layer * p.P.ks[0], p.P.ks) || !page_map(&vm, p.P, p.P.v + p.layer * p.P.vs[0], p.P.vs)) return cudaErrorNotSupported;
     const TcSize z = tc_size(p, n_sm);
@@ -1156,28 +1167,22 @@ cudaError_t launch_tc(const AttendParams &p, int n_sm, void *ws, long long wait_
     q.ml = (float *)((char *)ws + z.meta);
     q.part = (float *)((char *)ws + z.meta + z.ml);
     q.wait_limit = wait_limit;
-    // (the limit belongs to the kernel on the current device; setting it again costs a few hundred nanoseconds)
-    cudaError_t e = cudaFuncSetAttribute(attend_tc_kernel<D, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = launch_front(attend_tc_kernel<D, TY>, dim3(n_sm), TC_THREADS, smem, st, q, km, vm);
     if (e != cudaSuccess) return e;
-    attend_tc_kernel<D, TY><<<n_sm, TC_THREADS, smem, st>>>(q, km, vm);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(n_sm, (z.rows + 31) / 32);
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, attend_join_kernel<D, TY>, q);
+    e = launch_front(attend_join_kernel<D, TY>, dim3(n_sm, (z.rows + 31) / 32), 256, 0, st, q);
     if (e != cudaSuccess) return e;
     *launches += 2;
     return cudaGetLastError();
 }
 
 }  // namespace
+
+cudaError_t prepare_attend() {
+    for (cudaError_t e : {tc_prepare<64, PTY_F32>(), tc_prepare<64, PTY_F16>(), tc_prepare<64, PTY_BF16>(), tc_prepare<128, PTY_F32>(),
+                          tc_prepare<128, PTY_F16>(), tc_prepare<128, PTY_BF16>()})
+        if (e != cudaSuccess) return e;
+    return cudaSuccess;
+}
 
 size_t attend_ws_bytes(const AttendParams &p, int n_sm) {
     const TcSize z = tc_size(p, n_sm);

@@ -12,8 +12,10 @@ there is no CPU path here, and a missing library is an error, not a fallback.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import os
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -364,47 +366,82 @@ class KvCache:
         self._h = None
 
 
-# Device tensors (torch's, or anything with the same data_ptr / shape / stride / dtype / device) of the paged cache.
+# Device tensors (torch's, or anything with the same data_ptr / shape / stride / dtype / get_device) of the paged cache.
+# A serving loop makes these calls once a layer and token, so the checks are kept short and the requests are packed in
+# one go: an attend_pages call spends about as long here as a kernel launch takes.
+class _DtypeNames(dict):
+    """Type of a tensor -> its name: ``str`` of a dtype is slow, so each is asked once."""
+
+    def __missing__(self, dtype):
+        self[dtype] = name = str(dtype)
+        return name
+
+
+_DTYPE = _DtypeNames()
 _TENSOR_TY = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+_ATTEND_REQ = struct.Struct("@PIIPPQQQQIIPPIfiIPN0P")    # _AttendReq
+_ROPE_REQ = struct.Struct("@PIPIPPPPIQQQQQQQQIIPPIPPPf0P")   # _RopeReq
 
 
 def _tensor(t, what: str, shape, dtype: Optional[str], device: int, dense: bool = True):
     """Checks one device tensor argument: its device, dimensions (None: any size) and type; dense = C-contiguous."""
-    if t.device.type != "cuda" or t.device.index != device:
+    if t.get_device() != device:
         raise ValueError(f"{what} is on {t.device}, the context on cuda:{device}")
     if len(t.shape) != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape)):
         raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple('*' if w is None else w for w in shape)}")
-    if dtype is not None and str(t.dtype) != dtype:
+    if dtype is not None and _DTYPE[t.dtype] != dtype:
         raise ValueError(f"{what} is {t.dtype}, expected {dtype}")
     if dense and not t.is_contiguous():
         raise ValueError(f"{what} is not contiguous")
     return t
 
 
-def _rows(t, what: str, shape, device: int):
+def _ints(t, what: str, n: Optional[int], device: int) -> int:
+    """A contiguous vector of n (None: any number of) 32-bit integers on the device: its address."""
+    if t.get_device() != device or _DTYPE[t.dtype] != "torch.int32" or len(t.shape) != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+        _tensor(t, what, (n,), "torch.int32", device)
+    return t.data_ptr()
+
+
+def _rows(t, what: str, rows: Optional[int], heads: Optional[int], dim: int, device: int):
     """Rows of heads: any strides between rows and heads, the dimensions of a head next to one another."""
-    _tensor(t, what, shape, None, device, dense=False)
-    if str(t.dtype) not in _TENSOR_TY:
+    if t.get_device() != device:
+        raise ValueError(f"{what} is on {t.device}, the context on cuda:{device}")
+    ty = _TENSOR_TY.get(_DTYPE[t.dtype])
+    if ty is None:
         raise ValueError(f"{what} is {t.dtype}, expected float32, float16 or bfloat16")
-    if t.stride(2) != 1:
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or (rows is not None and shape[0] != rows) or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what} has shape {tuple(shape)}, expected ({rows or '*'}, {heads or '*'}, {dim})")
+    sr, sh, sd = t.stride()
+    if sd != 1:
         raise ValueError(f"{what}: the dimensions of a head are not contiguous")
-    return _TENSOR_TY[str(t.dtype)], (C.c_uint64 * 2)(t.stride(0), t.stride(1))
+    return ty, shape[0], shape[1], sr, sh
 
 
 def _stream(stream, t) -> int:
     """The cudaStream_t to work on: the caller's, or the current stream of the tensors' framework."""
-    if stream is not None:
-        return int(stream)
+    return _current_stream(t.get_device()) if stream is None else stream
+
+
+def _current_stream(device: int) -> int:
     import torch
 
-    return torch.cuda.current_stream(t.device).cuda_stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (what the line below costs 3 us to find out)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
-def _list32(a) -> np.ndarray:
+def _list32(a) -> bytes:
+    """A host list of 32-bit integers, as the C side reads it."""
+    if isinstance(a, (list, tuple, range)):
+        try:
+            return array.array("i", a).tobytes()
+        except (TypeError, OverflowError):
+            raise ValueError("sequence numbers and counts are 32-bit integers") from None
     a = np.asarray(a)
     if a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31):
         raise ValueError("sequence numbers and counts are 32-bit integers")
-    return np.ascontiguousarray(a.reshape(-1), dtype=np.int32)
+    return a.reshape(-1).astype(np.int32).tobytes()
 
 
 @dataclass
@@ -433,6 +470,7 @@ class Rope:
                 raise ValueError(f"{self._ff.size} frequency factors, expected {self.dim // 2}")
         self._c = _Rope(self.dim, ("half", "pairs").index(self.layout), ("none", "linear", "yarn").index(self.scaling), self.base,
                         self.factor, self.attn_factor, self.beta_fast, self.beta_slow, self.orig_ctx, _ptr(self._ff))
+        self._p = C.addressof(self._c)
 
 
 class KvPages:
@@ -452,7 +490,7 @@ class KvPages:
         _tensor(k, "k", (None,) * 5, None, dev, dense=False)
         L, NP, page, H, D = k.shape
         _tensor(v, "v", (L, NP, page, H, D), str(k.dtype), dev, dense=False)
-        if str(k.dtype) not in ("torch.float16", "torch.bfloat16"):
+        if _DTYPE[k.dtype] not in ("torch.float16", "torch.bfloat16"):
             raise ValueError(f"pages of {k.dtype}, expected float16 or bfloat16")
         if k.stride(4) != 1 or v.stride(4) != 1:
             raise ValueError("the dimensions of a head are not contiguous")
@@ -468,10 +506,22 @@ class KvPages:
         self.work = refs.new_zeros(64 + 4 * S + 3 * NP)
         #: what the last :meth:`Gpu.pages_reserve` reported, on the device: 0, the pages that were missing, or -1
         self.short_by = self.work[0]
-        self._c = _Pages(k.data_ptr(), v.data_ptr(), _TENSOR_TY[str(k.dtype)], L, NP, page, H, D,
+        self._c = _Pages(k.data_ptr(), v.data_ptr(), _TENSOR_TY[_DTYPE[k.dtype]], L, NP, page, H, D,
                          (C.c_uint64 * 4)(*k.stride()[:4]), (C.c_uint64 * 4)(*v.stride()[:4]), table.data_ptr(),
                          max(table.stride(0), W), S, W, lens.data_ptr(), refs.data_ptr(), self.work.data_ptr())
         self._p = C.addressof(self._c)
+        self._ws = {}
+
+    def _scratch(self, n: int, stream: Optional[int]):
+        """n bytes from the allocator of the tensors' framework, which may hand them on once the stream's work is done."""
+        n = (n + 3) // 4
+        if stream is not None:
+            import torch
+
+            if _current_stream(self.device) != stream:   # the allocator goes by the current stream
+                with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
+                    return self.work.new_empty(n)
+        return self.work.new_empty(n)
 
 
 class Gpu:
@@ -742,79 +792,93 @@ class Gpu:
             raise ValueError(f"the pool is on cuda:{pages.device}, the context on cuda:{self.device}")
         if not 0 <= layer < pages.n_layers:
             raise ValueError(f"layer {layer} of {pages.n_layers}")
-        n = _tensor(cu, "cu", (None,), "torch.int32", self.device).shape[0] - 1
+        at = _ints(cu, "cu", None, pages.device)
+        n = cu.shape[0] - 1
         if n < 0:
             raise ValueError("cu holds n + 1 row offsets")
-        if seqs is not None:
-            _tensor(seqs, "seqs", (n,), "torch.int32", self.device)
-        return n
+        return n, at, 0 if seqs is None else _ints(seqs, "seqs", n, pages.device)
 
     def rope_append(self, pages: KvPages, layer: int, q, k, v, cu, rope: Optional[Rope], out=None, seqs=None, positions=None,
                     q_norm=None, k_norm=None, eps: float = 1e-6, stream: Optional[int] = None, wait: bool = False) -> bool:
         """``apk_rope_append``: per-head norms and rotation of one layer's new rows; q goes to ``out`` (None: in place),
         k and v into the pages.  q [rows, heads, head_dim] (or None), k, v [rows, kv heads, head_dim]; rows
         ``cu[i]`` .. ``cu[i+1]-1`` are the last positions of sequence ``seqs[i]`` (None: i)."""
-        n, dev, D = self._batch(pages, layer, cu, seqs), self.device, pages.head_dim
-        ty, ks = _rows(k, "k", (None, pages.n_kv_heads, D), dev)
-        T = k.shape[0]
-        vty, vs = _rows(v, "v", (T, pages.n_kv_heads, D), dev)
-        qty, qs = (ty, (C.c_uint64 * 2)()) if q is None else _rows(q, "q", (T, None, D), dev)
+        n, cu_at, seqs_at = self._batch(pages, layer, cu, seqs)
+        dev, D, H = pages.device, pages.head_dim, pages.n_kv_heads
+        ty, T, _, k0, k1 = _rows(k, "k", None, H, D, dev)
+        vty, _, _, v0, v1 = _rows(v, "v", T, H, D, dev)
+        if q is None:
+            qty = oty = ty
+            heads = q0 = q1 = o0 = o1 = q_at = out_at = 0
+        else:
+            out = q if out is None else out
+            qty, _, heads, q0, q1 = _rows(q, "q", T, None, D, dev)
+            oty, _, _, o0, o1 = _rows(out, "out", T, heads, D, dev)
+            q_at, out_at = q.data_ptr(), out.data_ptr()
         if vty != ty or qty != ty:
             raise ValueError("q, k and v are of one type")
-        out = q if out is None else out
-        oty, os_ = (ty, (C.c_uint64 * 2)()) if q is None else _rows(out, "out", tuple(q.shape), dev)
-        if positions is not None:
-            _tensor(positions, "positions", (T,), "torch.int32", dev)
         for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
             if w is not None:
                 _tensor(w, what, (D,), "torch.float32", dev)
-        req = _RopeReq(pages._p, layer, None if rope is None else C.addressof(rope._c), ty,
-                       None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), None if q is None else out.data_ptr(), oty,
-                       qs, ks, vs, os_, 0 if q is None else q.shape[1], T, cu.data_ptr(),
-                       None if seqs is None else seqs.data_ptr(), n, None if positions is None else positions.data_ptr(),
-                       None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps)
-        return self._check(self._l.apk_rope_append(self._h, C.byref(req), _stream(stream, k), 1 if wait else 0))
+        req = _ROPE_REQ.pack(pages._p, layer, 0 if rope is None else rope._p, ty, q_at, k.data_ptr(), v.data_ptr(), out_at, oty,
+                             q0, q1, k0, k1, v0, v1, o0, o1, heads, T, cu_at, seqs_at, n,
+                             0 if positions is None else _ints(positions, "positions", T, dev),
+                             0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), eps)
+        return self._check(self._l.apk_rope_append(self._h, req, _stream(stream, k), 1 if wait else 0))
 
     def attend_pages(self, pages: KvPages, layer: int, q, cu, scale: float, out, seqs=None, causal: bool = True, window: int = 0,
                      workspace=None, stream: Optional[int] = None, wait: bool = False) -> bool:
         """``apk_attend_pages``: the batch's rows q [rows, heads, head_dim] over one layer of the pages, into ``out``; rows
-        ``cu[i]`` .. ``cu[i+1]-1`` are the last positions of sequence ``seqs[i]`` (None: i).  ``workspace``: a uint8 tensor of
-        ``apk_attend_pages_ws`` bytes, for this call alone while it runs; None takes one from the tensors' allocator."""
-        n, D = self._batch(pages, layer, cu, seqs), pages.head_dim
-        ty, qs = _rows(q, "q", (None, None, D), self.device)
-        oty, os_ = _rows(out, "out", tuple(q.shape), self.device)
+        ``cu[i]`` .. ``cu[i+1]-1`` are the last positions of sequence ``seqs[i]`` (None: i).  ``workspace``: a tensor of
+        ``apk_attend_pages_ws`` bytes, for this call alone while it runs; None takes one from the allocator of the tensors'
+        framework, on the call's stream."""
+        n, cu_at, seqs_at = self._batch(pages, layer, cu, seqs)
+        D, dev = pages.head_dim, pages.device
+        ty, T, heads, q0, q1 = _rows(q, "q", None, None, D, dev)
+        oty, _, _, o0, o1 = _rows(out, "out", T, heads, D, dev)
         if oty != ty:
             raise ValueError("out is of q's type")
-        if window < 0:
+        if not 0 <= window < 2**31:
             raise ValueError(f"a window of {window}")
-        req = _AttendReq(pages._p, layer, ty, q.data_ptr(), out.data_ptr(), qs, os_, q.shape[1], q.shape[0], cu.data_ptr(),
-                         None if seqs is None else seqs.data_ptr(), n, scale, 1 if causal else 0, window, None, 0)
-        need = self._l.apk_attend_pages_ws(self._h, C.byref(req))
-        if need:
-            if workspace is None:
-                workspace = pages.work.new_empty((need + 3) // 4)
-            elif workspace.device != q.device:
-                raise ValueError(f"workspace is on {workspace.device}")
-            req.ws, req.ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        return self._check(self._l.apk_attend_pages(self._h, C.byref(req), _stream(stream, q), 1 if wait else 0))
+        need = pages._ws.get((T, heads, ty))
+        if need is None:   # (depends on nothing but these and the pool)
+            need = self._l.apk_attend_pages_ws(self._h, _ATTEND_REQ.pack(
+                pages._p, layer, ty, q.data_ptr(), out.data_ptr(), q0, q1, o0, o1, heads, T, cu_at, seqs_at, n, scale,
+                1 if causal else 0, window, 0, 0))
+            if need:
+                if len(pages._ws) > 256:
+                    pages._ws.clear()
+                pages._ws[(T, heads, ty)] = need
+        if workspace is None:
+            ws_at, ws_bytes = 0, need
+            if need:
+                workspace = pages._scratch(need, stream)
+                ws_at = workspace.data_ptr()
+        elif workspace.get_device() != dev:
+            raise ValueError(f"workspace is on {workspace.device}")
+        else:
+            ws_at, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        req = _ATTEND_REQ.pack(pages._p, layer, ty, q.data_ptr(), out.data_ptr(), q0, q1, o0, o1, heads, T, cu_at, seqs_at, n, scale,
+                               1 if causal else 0, window, ws_at, ws_bytes)
+        return self._check(self._l.apk_attend_pages(self._h, req, _stream(stream, q), 1 if wait else 0))
 
     def pages_reserve(self, pages: KvPages, seqs, n_new, stream: Optional[int] = None, wait: bool = True) -> bool:
         """``apk_pages_reserve``: room for ``n_new[i]`` more positions in sequence ``seqs[i]`` (host lists).  False when pages are
         missing or a row of the table is too short, and then nothing has changed; with ``wait`` off ``pages.short_by`` says so."""
         a, b = self._lists(pages, seqs, n_new)
-        return self._check(self._l.apk_pages_reserve(self._h, pages._p, a.size, a.ctypes.data, b.ctypes.data,
+        return self._check(self._l.apk_pages_reserve(self._h, pages._p, len(a) // 4, a, b,
                                                      _stream(stream, pages.work), 1 if wait else 0))
 
     def pages_fork(self, pages: KvPages, src, dst, stream: Optional[int] = None) -> bool:
         """``apk_pages_fork``: sequence ``dst[i]`` becomes a second holder of ``src[i]``'s positions (host lists)."""
         a, b = self._lists(pages, src, dst)
-        return self._check(self._l.apk_pages_fork(self._h, pages._p, a.size, a.ctypes.data, b.ctypes.data,
+        return self._check(self._l.apk_pages_fork(self._h, pages._p, len(a) // 4, a, b,
                                                   _stream(stream, pages.work)))
 
     def pages_release(self, pages: KvPages, seqs, keep, stream: Optional[int] = None) -> bool:
         """``apk_pages_release``: sequence ``seqs[i]`` keeps its first ``keep[i]`` positions (host lists)."""
         a, b = self._lists(pages, seqs, keep)
-        return self._check(self._l.apk_pages_release(self._h, pages._p, a.size, a.ctypes.data, b.ctypes.data,
+        return self._check(self._l.apk_pages_release(self._h, pages._p, len(a) // 4, a, b,
                                                      _stream(stream, pages.work)))
 
     def pages_compact(self, pages: KvPages, page_map=None, stream: Optional[int] = None) -> bool:
@@ -830,8 +894,8 @@ class Gpu:
         if pages.device != self.device:
             raise ValueError(f"the pool is on cuda:{pages.device}, the context on cuda:{self.device}")
         a, b = _list32(a), _list32(b)
-        if a.size != b.size:
-            raise ValueError(f"lists of {a.size} and {b.size} entries")
+        if len(a) != len(b):
+            raise ValueError(f"lists of {len(a) // 4} and {len(b) // 4} entries")
         return a, b
 
     # -- parity instrumentation ----------------------------------------------

@@ -36,6 +36,9 @@ class Tensor:
     def stride(self, i=None):
         return self._stride if i is None else self._stride[i]
 
+    def get_device(self):
+        return self.device.index
+
     def is_contiguous(self):
         return self._dense
 
@@ -50,6 +53,8 @@ class Tensor:
 
     def new_zeros(self, n):
         return Tensor(n, dtype="int32")
+
+    new_empty = new_zeros
 
     def __getitem__(self, i):
         return Tensor(dtype="int32")
@@ -81,6 +86,7 @@ def test_struct_sizes_against_the_compiler(gpu, tmp_path):
     exe = tmp_path / "sz"
     subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)])
     got = [int(v) for v in subprocess.check_output([str(exe)]).split()]
+    assert (gpu._ATTEND_REQ.size, gpu._ROPE_REQ.size) == (C.sizeof(gpu._AttendReq), C.sizeof(gpu._RopeReq))
     assert got == [C.sizeof(gpu._Pages), C.sizeof(gpu._Rope), C.sizeof(gpu._RopeReq), C.sizeof(gpu._AttendReq), gpu._Pages.work.offset,
                    gpu._RopeReq.eps.offset, gpu._AttendReq.ws.offset, 64 + 4 * 3 + 3 * 10]
 
