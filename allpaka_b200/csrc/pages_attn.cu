@@ -320,25 +320,61 @@ __device__ __forceinline__ void tc_hide(const AttendParams &a, const SeqRows &s,
         if (!((see >> k) & 1u)) f[k] = -INFINITY;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+template <int N>
 __device__ __forceinline__ float tc_max(const float *f) {
     float mx[4] = {f[0], f[1], f[2], f[3]};
 #pragma unroll
-    for (int k = 4; k < 32; ++k) mx[k & 3] = fmaxf(mx[k & 3], f[k]);
-    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    for (int k = 4; k + 8 <= N; k += 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], f[k + 2 * i], f[k + 2 * i + 1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], f[N - 4 + i]);
+    return max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
 }
 
-// 32 scores into 16 columns of weights (and as many of their second parts); returns the weights' sum.
-template <bool BF>
+// Two 32-bit values at a time
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 one_by_one(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// N scores into N / 2 columns of weights; returns the weights' sum.
+template <int N, bool BF>
 __device__ __forceinline__ float tc_exp16(const float *f, float c, float off, uint32_t *w) {
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint64_t c2 = two(c, c), off2 = two(off, off);
+    uint64_t sum[2] = {0, 0};
 #pragma unroll
-    for (int k = 0; k < 32; k += 2) {
-        const float p0 = ex2(fmaf(f[k], c, off)), p1 = ex2(fmaf(f[k + 1], c, off));
-        sum[(k >> 1) & 3] += p0 + p1;
+    for (int k = 0; k < N; k += 2) {
+        const float2 x = one_by_one(fma2(two(f[k], f[k + 1]), c2, off2));
+        const float p0 = ex2(x.x), p1 = ex2(x.y);
+        sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], two(p0, p1));
         w[k >> 1] = pack16<BF>(p0, p1);
     }
-    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    const float2 t = one_by_one(add2(sum[0], sum[1]));
+    return t.x + t.y;
 }
+// (and their second parts)
 __device__ __forceinline__ float tc_exp32(const float *f, float c, float off, uint32_t *hi, uint32_t *lw) {
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -378,66 +414,51 @@ __device__ __forceinline__ void tc_rescale(uint32_t to, float by) {
     }
 }
 
-// A block of scores (TMEM columns at `ts`) becomes 16-bit weights in the same columns: chunk by chunk of 32, twice over (the
-// maximum first), since 128 scores in registers would leave too few for anything else.  The weights of a chunk lie where scores
-// have been read already.  m: what the weights refer to, l: their sum; `first`: there are no sums O yet.
-// A quarter (part >= 0): the thread weighs 32 of the positions.
+// A block of scores (TMEM columns at `ts`) becomes 16-bit weights in the same columns.  m: what the weights refer to, l: their sum;
+// `first`: there are no sums O yet.  A quarter (part >= 0): the thread weighs 32 of the positions.
+// 128 scores stay in registers from their one load on: reading them again chunk by chunk costs six trips to TMEM a block instead
+// of one (a 4096-row chunk over 8192 positions: 604 us).  For the same reason nothing here may spill: with this much shared memory
+// there is next to no L1 for it.
 template <int D, bool BF>
 __device__ __forceinline__ void tc_weights16(const AttendParams &a, const SeqRows &s, const TcRow &row, uint32_t ts, uint32_t to, int part, int pos, bool first,
                                              float c, float &m, float &l) {
-    uint32_t xa[32], xb[32], w[16];
-    float *const fa = (float *)xa, *const fb = (float *)xb;
-    const int p0 = part < 0 ? pos : pos + part * 32;
-    const bool edge = row.odd || __any_sync(~0u, row.mine && (p0 < row.lo || p0 + (part < 0 ? 128 : 32) > row.hi));
-    float mx;
-    if (part >= 0) {
-        tm_ld(ts + part * 32, xa);
-        if (edge) tc_hide(a, s, row, p0, fa);
-        mx = tc_max(fa);
-    } else {
-        mx = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < 128; h += 64) {
-            tm_ld32(ts + h, xa);
-            tm_ld32(ts + h + 32, xb);
-            tm_wait_ld();
-            pin32(xa);
-            pin32(xb);
-            if (edge) { tc_hide(a, s, row, pos + h, fa); tc_hide(a, s, row, pos + h + 32, fb); }
-            mx = fmaxf(mx, fmaxf(tc_max(fa), tc_max(fb)));
+    const float shift = BF ? 0.f : 7.f;
+    auto moved = [&](float mx) {      // a row's maximum, and what becomes of m, l and O
+        mx *= c;
+        const bool grow = row.mine && mx > m + TC_LAZY;      // (from -inf: with the first visible position)
+        if (__any_sync(~0u, grow)) {
+            const float to_m = grow ? mx : m;
+            const float by = m == -INFINITY ? 0.f : ex2(m - to_m);
+            m = to_m;
+            l *= by;
+            // (this group's products so far are complete: they were issued before the scores)
+            if (!first) tc_rescale<D>(to, by);
         }
-        tm_ld32(ts, xa);
-    }
-    mx *= c;
-    const bool grow = row.mine && mx > m + TC_LAZY;      // (from -inf: with the first visible position)
-    if (__any_sync(~0u, grow)) {
-        const float to_m = grow ? mx : m;
-        const float by = m == -INFINITY ? 0.f : ex2(m - to_m);
-        m = to_m;
-        l *= by;
-        // (this group's products so far are complete: they were issued before the scores)
-        if (!first) tc_rescale<D>(to, by);
-    }
-    const float off = (BF ? 0.f : 7.f) - (m == -INFINITY ? 0.f : m);
+        return shift - (m == -INFINITY ? 0.f : m);
+    };
     if (part >= 0) {
-        l += tc_exp16<BF>(fa, c, off, w);
+        uint32_t x[32], w[16];
+        float *const f = (float *)x;
+        const int p0 = pos + part * 32;
+        tm_ld(ts + part * 32, x);
+        if (row.odd || __any_sync(~0u, row.mine && (p0 < row.lo || p0 + 32 > row.hi))) tc_hide(a, s, row, p0, f);
+        const float off = moved(tc_max<32>(f));
+        l += tc_exp16<32, BF>(f, c, off, w);
         tc_put_quarter(ts, part, w);
     } else {
+        uint32_t x[128], w[64];
+        float *const f = (float *)x;
+        tm_ld32(ts, x); tm_ld32(ts + 32, x + 32); tm_ld32(ts + 64, x + 64); tm_ld32(ts + 96, x + 96);
+        tm_wait_ld();
+        pin32(x); pin32(x + 32); pin32(x + 64); pin32(x + 96);
+        if (row.odd || __any_sync(~0u, row.mine && (pos < row.lo || pos + 128 > row.hi))) {
 #pragma unroll
-        for (int h = 0; h < 128; h += 64) {
-            tm_wait_ld();
-            pin32(xa);
-            tm_ld32(ts + h + 32, xb);
-            if (edge) tc_hide(a, s, row, pos + h, fa);
-            l += tc_exp16<BF>(fa, c, off, w);
-            tm_st16(ts + h / 2, w);
-            tm_wait_ld();
-            pin32(xb);
-            if (h == 0) tm_ld32(ts + 64, xa);
-            if (edge) tc_hide(a, s, row, pos + h + 32, fb);
-            l += tc_exp16<BF>(fb, c, off, w);
-            tm_st16(ts + h / 2 + 16, w);
+            for (int h = 0; h < 128; h += 32) tc_hide(a, s, row, pos + h, f + h);
         }
+        const float off = moved(tc_max<128>(f));
+        l += tc_exp16<128, BF>(f, c, off, w);
+        tm_st32(ts, w);
+        tm_st32(ts + 32, w + 32);
     }
     tm_wait_st();
 }
@@ -452,13 +473,13 @@ __device__ __forceinline__ float tc_weights32(const AttendParams &a, const SeqRo
     if (part >= 0) {
         tm_ld(ts + part * 32, x);
         if (edge) tc_hide(a, s, row, p0, f);
-        mx = tc_max(f);
+        mx = tc_max<32>(f);
     } else {
 #pragma unroll
         for (int h = 0; h < 128; h += 32) {
             tm_ld(ts + h, x);
             if (edge) tc_hide(a, s, row, pos + h, f);
-            mx = fmaxf(mx, tc_max(f));
+            mx = fmaxf(mx, tc_max<32>(f));
         }
     }
     const float to_m = fmaxf(m, mx * c);
