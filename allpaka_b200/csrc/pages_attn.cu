@@ -614,60 +614,73 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
             // every copy that was asked for has arrived before the block ends
             for (int idx = max(0, filled - TC_STAGES); idx < filled; ++idx)
                 (void)mbar_wait_bounded(&sh.full[idx % TC_STAGES], (idx / TC_STAGES) & 1, p.wait_limit);
-        } else if (warp == 9 && lane == 0) {
-            // -------------------------------------------------------- tensor instructions: one thread
+        } else if (warp == 9) {
+            // -------------------------------------------------------- tensor instructions: issued by one thread of a warp that stays
+            // together, so that their operands are the warp's and not the thread's (one thread alone took 85 cycles for each)
+            const bool leader = elect_one();
             uint32_t ph_q = 0, ph_p = 0;
             const uint32_t q_addr = smem_u32(qs), r_addr = smem_u32(ring);
-            while ((ok = seg_wait())) {
-                const int n = segment().n;
+            while ((ok = __all_sync(~0u, seg_wait()))) {
+                const int n = __shfl_sync(~0u, segment().n, 0);
                 if (n < 0) break;
-                const bool wide = !F32 && segment().ntok > tq;
-                mbar_arrive(&sh.seg_empty[n_seg % TC_SEGS]);
+                const bool wide = !F32 && __shfl_sync(~0u, segment().ntok, 0) > tq;
+                __syncwarp();
+                if (leader) mbar_arrive(&sh.seg_empty[n_seg % TC_SEGS]);
                 ++n_seg;
                 if (n == 0) continue;
-                if (!(ok = tc_wait(sh, &sh.q_full, ph_q, p, 4))) break;
+                if (!(ok = __all_sync(~0u, tc_wait(sh, &sh.q_full, ph_q, p, 4)))) break;
                 ph_q ^= 1;
                 // Step i is the product with V of one group and the scores of its next block: wide, both groups for every block (group
                 // i & 1, block i / 2); narrow, the groups in turn (block i).  The first two steps have scores only.
                 const int steps = wide ? 2 * n : n;
+#pragma unroll 1
                 for (int i = -2; i < steps; ++i) {
                     const int w = i & 1;
                     const bool last = i + 2 >= steps, both = !wide || w;   // both: no other group needs the block any more
                     if (i >= 0) {
                         const int v = ring0 + tc_slot_v(wide, wide ? i >> 1 : i, n), st = v % TC_STAGES;
-                        if (!(ok = tc_wait(sh, &sh.full[st], (v / TC_STAGES) & 1, p, 2) && tc_wait(sh, &sh.p_full[w], ph_p >> w & 1, p, 3))) break;
+                        if (!(ok = __all_sync(~0u, tc_wait(sh, &sh.full[st], (v / TC_STAGES) & 1, p, 2) && tc_wait(sh, &sh.p_full[w], ph_p >> w & 1, p, 3)))) break;
                         ph_p ^= 1u << w;
                         tc_fence_after();
-                        const uint32_t va = r_addr + st * TILE;
-                        const bool add = !F32 && i > 1;
+                        if (leader) {
+                            const uint64_t va = tc_desc(r_addr + st * TILE, TC_BLOCK * 128);
+                            const uint32_t o = tmem + O_COL + w * D, pw = tmem + w * 128;
+                            const bool add = !F32 && i > 1;
 #pragma unroll
-                        for (int part = PARTS - 1; part >= 0; --part)
+                            for (int part = PARTS - 1; part >= 0; --part)
 #pragma unroll
-                            for (int k = 0; k < TC_BLOCK / 16; ++k)
-                                tc_mma_ts(tmem + O_COL + w * D, tmem + w * 128 + part * 64 + k * 8, tc_desc(va + k * 2048, TC_BLOCK * 128), idesc_pv,
-                                          add || part < PARTS - 1 || k > 0);
-                        if (both) tc_commit(&sh.empty[st]);
-                        if (F32 || last) tc_commit(&sh.o_full[w]);
+                                for (int k = 0; k < TC_BLOCK / 16; ++k)
+                                    tc_mma_ts(o, pw + part * 64 + k * 8, va + (uint64_t)(k * 2048 >> 4), idesc_pv, add || part < PARTS - 1 || k > 0);
+                            if (both) tc_commit(&sh.empty[st]);
+                            if (F32 || last) tc_commit(&sh.o_full[w]);
+                        }
                     }
                     if (!last) {
                         const int kn = ring0 + tc_slot_k(wide, wide ? (i + 2) >> 1 : i + 2), st = kn % TC_STAGES;
-                        if (!(ok = tc_wait(sh, &sh.full[st], (kn / TC_STAGES) & 1, p, 2))) break;
+                        if (!(ok = __all_sync(~0u, tc_wait(sh, &sh.full[st], (kn / TC_STAGES) & 1, p, 2)))) break;
                         tc_fence_after();
-                        const uint32_t qa = q_addr + (wide ? w * TILE : 0), ka = r_addr + st * TILE;
-                        // (low parts first: a sum is truncated where it is, and theirs are small)
+                        if (leader) {
+                            const uint64_t qa = tc_desc(q_addr + (wide ? w * TILE : 0), 16), ka = tc_desc(r_addr + st * TILE, 16);
+                            const uint32_t d = tmem + w * 128;
+                            // (low parts first: a sum is truncated where it is, and theirs are small)
 #pragma unroll
-                        for (int part = PARTS - 1; part >= 0; --part)
+                            for (int part = PARTS - 1; part >= 0; --part)
 #pragma unroll
-                            for (int k = 0; k < D / 16; ++k) {
-                                const uint32_t off = (k >> 2) * (TC_BLOCK * 128) + (k & 3) * 32;
-                                tc_mma_ss(tmem + w * 128, tc_desc(qa + part * TILE + off, 16), tc_desc(ka + off, 16), idesc_qk, part < PARTS - 1 || k > 0);
-                            }
-                        tc_commit(&sh.s_full[w]);
-                        if (both) tc_commit(&sh.empty[st]);
+                                for (int k = 0; k < D / 16; ++k) {
+                                    const uint32_t off = (k >> 2) * (TC_BLOCK * 128) + (k & 3) * 32;
+                                    tc_mma_ss(d, qa + (uint64_t)((part * TILE + off) >> 4), ka + (uint64_t)(off >> 4), idesc_qk, part < PARTS - 1 || k > 0);
+                                }
+                            tc_commit(&sh.s_full[w]);
+                            if (both) tc_commit(&sh.empty[st]);
+                        }
                     }
                 }
                 if (!ok) break;
                 ring0 += 2 * n;
+            }
+            if (leader) {
+                tc_commit(&sh.drain);
+                (void)mbar_wait_bounded(&sh.drain, 0, p.wait_limit);
             }
         } else if (warp == 10) {
             // ------------------------------------------------------- units of every sequence, their running sum, the CTA's segments
@@ -1044,11 +1057,6 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
     __syncthreads();
     if (tid == 0) p.meta[cta * 8 + 6] = sh.odd;
     if (warp == 9) {
-        if (lane == 0) {
-            tc_commit(&sh.drain);
-            (void)mbar_wait_bounded(&sh.drain, 0, p.wait_limit);
-        }
-        __syncwarp();
         tc_fence_after();
         tm_dealloc(tmem, 512);
     }
