@@ -174,10 +174,12 @@ __host__ __device__ __forceinline__ void tc_next(const TcBatch &c, TcTile &x) {
     tc_open(c, x);
 }
 
-// Where the cut before unit u falls: a tile and a block.  A cut that would leave a single block on one side moves to
-// the tile's edge.
-__host__ __device__ inline void tc_cut(const TcBatch &c, const int *prefix, int total, int u, int *out) {
-    TcTile x;
+// Fewest blocks of a piece of a cut tile: its rows are loaded, stored and joined once more, which costs a narrow tile about one
+// block's time and a wide one (up to 256 rows of partial sums) three.
+__host__ __device__ __forceinline__ int tc_edge(const TcBatch &c, const TcTile &x) { return x.ntok > c.tq ? 4 : 2; }
+
+// Where the cut before unit u falls: a tile and a block of it (returned).  A cut too near to a tile's edge moves there.
+__host__ __device__ inline int tc_cut(const TcBatch &c, const int *prefix, int total, int u, TcTile &x) {
     x.t = x.h = 0;
     int block = 0;
     if (u >= total) {
@@ -201,40 +203,35 @@ __host__ __device__ inline void tc_cut(const TcBatch &c, const int *prefix, int 
         x.h = (u - x.base) / (x.nb + TC_OVERHEAD);
         x.base += x.h * (x.nb + TC_OVERHEAD);
         block = u - x.base - TC_OVERHEAD;
-        if (u == x.base || block <= 1) {
+        if (u == x.base || block < tc_edge(c, x)) {
             block = 0;
-        } else if (block >= x.nb - 1) {
+        } else if (block > x.nb - tc_edge(c, x)) {
             tc_next(c, x);
             block = 0;
         }
     }
-    out[0] = x.seq; out[1] = x.t; out[2] = x.h; out[3] = block; out[4] = x.base;
+    return block;
 }
 
 // The segments of a CTA's range, in order.
 struct TcWalk {
     TcTile x;
-    int j0, j1;   // blocks of the tile
-    __host__ __device__ __forceinline__ bool check(const TcBatch &c, const int *end) {
+    int j0, j1;                      // blocks of the tile
+    int e_seq, e_t, e_h, e_block;    // where the range ends
+    __host__ __device__ __forceinline__ bool check(const TcBatch &c) {
         if (x.seq >= c.p.B.n) return false;
-        if (x.seq == end[0] && x.t == end[1] && x.h == end[2]) {
-            j1 = end[3];
+        if (x.seq == e_seq && x.t == e_t && x.h == e_h) {
+            j1 = e_block;
             return j1 > j0;
         }
         j1 = x.nb;
-        return x.seq < end[0] || (x.seq == end[0] && (x.t < end[1] || (x.t == end[1] && x.h < end[2])));
+        return x.seq < e_seq || (x.seq == e_seq && (x.t < e_t || (x.t == e_t && x.h < e_h)));
     }
-    __host__ __device__ __forceinline__ bool start(const TcBatch &c, const int *begin, const int *end) {
-        x.seq = begin[0]; x.t = begin[1]; x.h = begin[2]; x.base = begin[4];
-        j0 = begin[3];
-        tc_open(c, x);
-        return check(c, end);
-    }
-    __host__ __device__ __forceinline__ bool next(const TcBatch &c, const int *end) {
-        if (x.seq == end[0] && x.t == end[1] && x.h == end[2]) return false;
+    __host__ __device__ __forceinline__ bool next(const TcBatch &c) {
+        if (x.seq == e_seq && x.t == e_t && x.h == e_h) return false;
         tc_next(c, x);
         j0 = 0;
-        return check(c, end);
+        return check(c);
     }
 };
 
@@ -250,7 +247,6 @@ struct TcShared {
     uint64_t full[TC_STAGES], empty[TC_STAGES], seg_full[TC_SEGS], seg_empty[TC_SEGS], q_full, s_full[2], p_full[2], o_full[2], o_free[2], both, half, drain;
     uint32_t tmem;
     int dead, odd;          // a wait ran out; a result is not finite
-    int cut[2][8];          // where the CTA's range begins and ends: sequence, tile, head, block, and the tile's first unit
     int gone[2][8];         // per warp: a page of the segment is not there
     float ml[128][2];       // maxima and sums that one softmax group hands to the other
     float red[128][2];      // ... and the lanes of one group to one another
@@ -543,6 +539,10 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
         fence_mbar_init();
     }
     if (warp == 9) tm_alloc(&sh.tmem, 512);
+    if (tid == 256) {
+        tma_prefetch_map(&kmap);
+        tma_prefetch_map(&vmap);
+    }
     pages_wait_front();
     for (int i = tid; i < min(a.B.n, TC_INFO); i += TC_THREADS) sh.info[i] = batch_seq(a.P, a.B, i);
     tc_fence_before();
@@ -686,48 +686,48 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
             // ------------------------------------------------------- units of every sequence, their running sum, the CTA's segments
             const TcBatch g(a, sh.info);
             const int seqs = a.B.n;
-            const bool lanes = seqs < 32;  // few sequences: the lanes over a sequence's tiles; many: a lane each
             int total = 0;
             if (lane == 0) sh.prefix[0] = 0;
 #pragma unroll 1
-            for (int i0 = 0; i0 < seqs; i0 += lanes ? 1 : 32) {
-                const int i = lanes ? i0 : i0 + lane;
+            for (int i0 = 0; i0 < seqs; i0 += 32) {   // a lane a sequence
+                const int i = i0 + lane;
                 int units = 0;
                 if (i < seqs) {
                     TcTile x;
                     x.s = g.seq(i);
-                    const int nt = (x.s.rows + g.step - 1) / g.step;
 #pragma unroll 1
-                    for (x.t = lanes ? lane : 0; x.t < nt; x.t += lanes ? 32 : 1) {
+                    for (x.t = 0; x.t * g.step < x.s.rows; ++x.t) {
                         tc_span(g, x);
                         units = min(units + x.nb + TC_OVERHEAD, TC_MOST);
                     }
                 }
-                if (lanes)
-                    for (int o = 16; o; o >>= 1) units = min(units + __shfl_xor_sync(~0u, units, o), TC_MOST);
                 units = (int)min((long long)units * a.P.kv, (long long)TC_MOST);
-                if (!lanes)
+                if (seqs > 1)
                     for (int o = 1; o < 32; o <<= 1) {
                         const int y = __shfl_up_sync(~0u, units, o);
                         if (lane >= o) units = min(units + y, TC_MOST);
                     }
                 units = min(total + units, TC_MOST);
-                if (i < seqs && (!lanes || lane == 0)) sh.prefix[i + 1] = units;
-                total = __shfl_sync(~0u, units, 31);
+                if (i < seqs) sh.prefix[i + 1] = units;
+                total = __shfl_sync(~0u, units, seqs > 1 ? 31 : 0);
             }
             __syncwarp();
             // (offsets that overlap could claim more rows than there are: such a batch is left alone)
             if (total >= TC_MOST) total = 0;
             const int per = max((int)(((long long)total + p.n_ctas - 1) / p.n_ctas), TC_MIN_UNITS);
-            if (lane < 2) {
-                const long long u = (long long)(cta + lane) * per;
-                tc_cut(g, sh.prefix, total, (int)(u < total ? u : total), sh.cut[lane]);
+            // lane 0 finds where the range begins, lane 1 where it ends
+            TcWalk wk;
+            {
+                const long long u = (long long)(cta + (lane & 1)) * per;
+                wk.j0 = tc_cut(g, sh.prefix, total, (int)(u < total ? u : total), wk.x);
+                wk.e_seq = __shfl_sync(~0u, wk.x.seq, 1);
+                wk.e_t = __shfl_sync(~0u, wk.x.t, 1);
+                wk.e_h = __shfl_sync(~0u, wk.x.h, 1);
+                wk.e_block = __shfl_sync(~0u, wk.j0, 1);
             }
-            __syncwarp();
             if (lane == 0) {
-                TcWalk wk;
                 int cuts = 0;
-                bool more = wk.start(g, sh.cut[0], sh.cut[1]);
+                bool more = wk.check(g);
 #pragma unroll 1
                 for (;;) {
                     const int at = n_seg % TC_SEGS;
@@ -742,13 +742,13 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                     if (!more) break;
                     // the first of a cut tile's pieces says how many follow: the cuts that stay inside the tile
                     if (wk.j0 == 0 && wk.j1 < wk.x.nb) {
-                        const int lo = wk.x.base + TC_OVERHEAD + 2, hi = wk.x.base + TC_OVERHEAD + wk.x.nb - 2;
+                        const int edge = tc_edge(g, wk.x), lo = wk.x.base + TC_OVERHEAD + edge, hi = wk.x.base + TC_OVERHEAD + wk.x.nb - edge;
                         int *mt = p.meta + cta * 8;
                         cuts = hi / per - (lo - 1) / per;
                         mt[1] = wk.x.s.first + wk.x.tok0; mt[2] = wk.x.ntok; mt[3] = wk.x.h; mt[4] = !F32 && wk.x.ntok > tq;
                     }
                     ++n_seg;
-                    more = wk.next(g, sh.cut[1]);
+                    more = wk.next(g);
                 }
                 p.meta[cta * 8] = cuts;
             }
@@ -1062,75 +1062,72 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
     }
 }
 
+// The heads of row t whose results are not finite, done over position by position.
+template <int D, typename T, typename C>
+__device__ __noinline__ void attend_mend(const AttendParams &a, int t, int warp, int lane) {
+    constexpr int E = D / 32;
+    const int i = batch_find(a.B, t);
+    if (i < 0) return;
+    const SeqRows s = batch_seq(a.P, a.B, i);
+    for (int hd = warp; hd < a.heads; hd += 8) {
+        const T *o = (const T *)a.out + t * a.os[0] + hd * a.os[1] + lane * E;
+        float size = 0.f;
+        for (int e = 0; e < E; ++e) size += fabsf(to_f32(o[e]));
+        if (__any_sync(~0u, !(size < INFINITY))) attend_row<D, T, C>(a, s, t, hd, lane);
+    }
+}
+
 // Merges the pieces of a cut tile: block c those of the tile whose first piece CTA c has left.  Piece 0 lies in slot 1 of CTA c,
 // the others in slot 0 of the CTAs behind it.  A warp per row, in the order of the pieces.
 // An infinity or NaN in V at a position that some rows of a tile do not see has met their weight of 0 in the product.  Such
 // rows show it by not being finite; they are done over here, position by position.
 template <int D, int TY>
-__global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ TcParams p) {
-    constexpr int E = D / 32;
+__global__ void __launch_bounds__(256, 4) attend_join_kernel(const __grid_constant__ TcParams p) {
+    constexpr int LANES = D / 4, ROWS = 32 / LANES;   // lanes a row, four values each; rows a warp
     typedef typename Elem<TY>::T T;
     typedef typename Elem<TY == PTY_BF16 ? PTY_BF16 : PTY_F16>::T C;
     const AttendParams &a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pages_let_next();
     pages_wait_front();
-    const int *mt = p.meta + blockIdx.x * 8;
-    const int more = mt[0], row0 = mt[1], ntok = mt[2], h = mt[3], wide = mt[4];
+    const int4 mt = *(const int4 *)(p.meta + blockIdx.x * 8);
+    const int more = mt.x, row0 = mt.y, ntok = mt.z, h = mt.w;
     int odd = 0;
-    for (int i = threadIdx.x; i < p.n_ctas; i += blockDim.x) odd |= p.meta[i * 8 + 6];
-    auto over = [&](int t, int hd) {
-        const int i = batch_find(a.B, t);
-        if (i >= 0) attend_row<D, T, C>(a, batch_seq(a.P, a.B, i), t, hd, lane);
-    };
-    if (__syncthreads_or(odd)) {
-        for (int t = blockIdx.y * gridDim.x + blockIdx.x; t < a.B.rows; t += gridDim.x * gridDim.y)
-            for (int hd = warp; hd < a.heads; hd += 8) {
-                const T *o = (const T *)a.out + t * a.os[0] + hd * a.os[1] + lane * E;
-                float size = 0.f;
-                for (int e = 0; e < E; ++e) size += fabsf(to_f32(o[e]));
-                if (__any_sync(~0u, !(size < INFINITY))) over(t, hd);
-            }
-    }
-    if (more <= 0 || more >= p.n_ctas - (int)blockIdx.x) return;
-    const int tq = 128 / a.group, n_rows = wide ? 128 + (ntok - tq) * a.group : ntok * a.group;
-    for (int r = blockIdx.y * 8 + warp; r < n_rows; r += 8 * gridDim.y) {
-        const int half = r >> 7, rr = r & 127, tok = (wide ? half * tq : 0) + rr / a.group;
-        if (rr >= tq * a.group || tok >= ntok) continue;
-        auto at = [&](int piece) { return (long long)(piece ? 2 * ((int)blockIdx.x + piece) : 2 * (int)blockIdx.x + 1) * p.ws_rows + r; };
-        float top = -INFINITY, l = 0.f, o[E];
-        for (int i = lane; i <= more; i += 32) top = fmaxf(top, p.ml[at(i) * 2]);
-        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-        for (int e = 0; e < E; ++e) o[e] = 0.f;
-        for (int i0 = 0; i0 <= more; i0 += 32) {
-            float b = 0.f, lb = 0.f;   // lane i: the weight of piece i0 + i
-            if (i0 + lane <= more) {
-                const float2 ml = *(const float2 *)(p.ml + at(i0 + lane) * 2);
-                if (ml.x != -INFINITY) { b = ex2(ml.x - top); lb = b * ml.y; }
-            }
-            l += lb;
-            const int n = min(32, more + 1 - i0);
+    for (int i = threadIdx.x; i < p.n_ctas; i += 256) odd |= p.meta[i * 8 + 6];
+    if (more > 0 && more < p.n_ctas - (int)blockIdx.x) {
+        const int tq = 128 / a.group;
+        const bool wide = TY != PTY_F32 && ntok > tq;
+        const int n_rows = wide ? 128 + (ntok - tq) * a.group : ntok * a.group, sub = lane / LANES, ch = lane % LANES;
+#pragma unroll 1
+        for (int r0 = (blockIdx.y * 8 + warp) * ROWS; r0 < n_rows; r0 += 8 * ROWS * gridDim.y) {
+            const int r = min(r0 + sub, n_rows - 1), rr = r & 127, tok = (r >= 128 ? tq : 0) + rr / a.group;
+            const bool mine = r0 + sub < n_rows && rr < tq * a.group;
+            auto at = [&](int piece) { return (2 * ((int)blockIdx.x + piece) + (piece == 0)) * p.ws_rows + r; };
+            float top = -INFINITY, l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = ch; i <= more; i += LANES) top = fmaxf(top, p.ml[(long long)at(i) * 2]);
+#pragma unroll
+            for (int x = LANES / 2; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
 #pragma unroll 4
-            for (int i = 0; i < n; ++i) {
-                const float bi = __shfl_sync(~0u, b, i);
-                const float *src = p.part + at(i0 + i) * D + lane * E;
-                float v[E];
-                if constexpr (E == 4) *(float4 *)v = *(const float4 *)src;
-                else *(float2 *)v = *(const float2 *)src;
-                for (int e = 0; e < E; ++e) o[e] = fmaf(bi, v[e], o[e]);
+            for (int i = 0; i <= more; ++i) {
+                const float2 ml = *(const float2 *)(p.ml + (long long)at(i) * 2);
+                const float4 v = *(const float4 *)(p.part + (long long)at(i) * D + ch * 4);
+                const float b = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+                l = fmaf(b, ml.y, l);
+                o.x = fmaf(b, v.x, o.x); o.y = fmaf(b, v.y, o.y); o.z = fmaf(b, v.z, o.z); o.w = fmaf(b, v.w, o.w);
             }
+            const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+            o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+            const int row = row0 + tok, head = h * a.group + rr % a.group;
+            if (mine) put4<TY>(a.out, row * a.os[0] + head * a.os[1] + ch * 4, o);
+            if (__any_sync(~0u, mine && !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY))) odd = 1;
         }
-        for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(~0u, l, x);
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        float size = 0.f;
-        for (int e = 0; e < E; ++e) { o[e] *= inv; size += fabsf(o[e]); }
-        const int row = row0 + tok, head = h * a.group + rr % a.group;
-        T *out = (T *)a.out + row * a.os[0] + head * a.os[1] + lane * E;
-        for (int e = 0; e < E; ++e) from_f32(out + e, o[e]);
-        if (__any_sync(~0u, !(size < INFINITY))) {
-            __syncwarp();
-            over(row, head);
-        }
+    }
+    // (the rows of other blocks' tiles may still be on their way to `out`: each block looks at its own tile's and at whole tiles')
+    if (__syncthreads_or(odd)) {
+        for (int t = blockIdx.y * gridDim.x + blockIdx.x; t < a.B.rows; t += gridDim.x * gridDim.y) attend_mend<D, T, C>(a, t, warp, lane);
+        if (more > 0)
+            for (int t = row0 + (int)blockIdx.y; t < row0 + ntok; t += gridDim.y) attend_mend<D, T, C>(a, t, warp, lane);
     }
 }
 

@@ -71,6 +71,7 @@ __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t *r) {
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void tma_prefetch_map(const void *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 // One box of a 4-dimensional tensor map: (dimension, position of a page, kv head, page).  x is a multiple of 64 elements.
 __device__ __forceinline__ void tma_load_4d(void *dst, const void *map, int x, int y, int z, int w, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
