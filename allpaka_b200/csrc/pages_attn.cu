@@ -106,8 +106,11 @@ __device__ __noinline__ void attend_row(const AttendParams &p, const SeqRows &s,
 constexpr int TC_THREADS = 384;      // warps 0-7 softmax, 8 copies, 9 tensor instructions, 10 walks the segments, 11 completes the third register group
 constexpr int TC_STAGES = 4;
 constexpr int TC_BLOCK = 128;         // positions a block
-constexpr int TC_OVERHEAD = 2;        // what opening and closing a tile costs, in blocks
-constexpr int TC_MIN_UNITS = 4;       // least range of a CTA
+// Units of work: a block of a narrow tile is one, of a wide tile two; opening and closing a tile costs as much as TC_OPEN blocks of
+// its own.   (64 sessions of 200 to 8192 positions: 122 us with 2, 116 with 3, 109 with 4, 110 with 6; a 4096-row chunk 454, 454, 447, 443.)
+constexpr int TC_OPEN = 4;
+constexpr int TC_MIN_UNITS = 2;       // least range of a CTA
+constexpr int TC_FEW = 4;             // fewer units a CTA than this, without the opening: it is not counted, so that all CTAs have a share
 constexpr int TC_MOST = 1 << 30;      // units of a call (the host has bounded a proper batch's)
 constexpr int TC_SEGS = 4;            // segments that are known ahead
 constexpr int TC_INFO = 256;          // sequences that a block keeps a copy of
@@ -127,6 +130,7 @@ struct TcBatch {
     const AttendParams &p;
     int tq, step;           // tokens per 128 rows, per tile
     const SeqRows *info;    // the first TC_INFO sequences, where a copy is at hand
+    int open = TC_OPEN;     // blocks that opening a tile counts for
     __host__ __device__ __forceinline__ TcBatch(const AttendParams &p_, const SeqRows *i)
         : p(p_), tq(128 / p_.group), step(p_.ty == PTY_F32 ? 128 / p_.group : 2 * (128 / p_.group)), info(i) {}
     __host__ __device__ __forceinline__ SeqRows seq(int i) const { return info && i < TC_INFO ? info[i] : batch_seq(p.P, p.B, i); }
@@ -138,6 +142,8 @@ struct TcTile {
     int nt;                 // tiles of the sequence
     SeqRows s;
     int tok0, ntok, k0, nb; // first token (of the sequence), tokens, first block, blocks
+    int per_block, opening; // units
+    __host__ __device__ __forceinline__ int units() const { return nb * per_block + opening; }
 };
 
 __host__ __device__ __forceinline__ void tc_span(const TcBatch &c, TcTile &x) {
@@ -149,6 +155,8 @@ __host__ __device__ __forceinline__ void tc_span(const TcBatch &c, TcTile &x) {
     row_span(c.p, x.s.len, pos + x.ntok - 1, unused, hi);
     x.k0 = lo / TC_BLOCK;
     x.nb = hi > lo ? (hi + TC_BLOCK - 1) / TC_BLOCK - x.k0 : 0;
+    x.per_block = x.ntok > c.tq ? 2 : 1;
+    x.opening = max(c.open * x.per_block, x.nb == 0 ? 1 : 0);   // (a tile without blocks has its rows to clear)
 }
 
 __host__ __device__ __forceinline__ void tc_open(const TcBatch &c, TcTile &x) {
@@ -162,7 +170,7 @@ __host__ __device__ __forceinline__ void tc_open(const TcBatch &c, TcTile &x) {
 }
 
 __host__ __device__ __forceinline__ void tc_next(const TcBatch &c, TcTile &x) {
-    x.base += x.nb + TC_OVERHEAD;
+    x.base += x.units();
     if (++x.h < c.p.P.kv) return;
     x.h = 0;
     if (++x.t < x.nt) {
@@ -195,15 +203,15 @@ __host__ __device__ inline int tc_cut(const TcBatch &c, const int *prefix, int t
         x.seq = lo;
         x.base = prefix[lo];
         tc_open(c, x);
-        while ((long long)x.base + (long long)(x.nb + TC_OVERHEAD) * c.p.P.kv <= u) {
-            x.base += (x.nb + TC_OVERHEAD) * c.p.P.kv;
+        while ((long long)x.base + (long long)x.units() * c.p.P.kv <= u) {
+            x.base += x.units() * c.p.P.kv;
             ++x.t;
             tc_span(c, x);
         }
-        x.h = (u - x.base) / (x.nb + TC_OVERHEAD);
-        x.base += x.h * (x.nb + TC_OVERHEAD);
-        block = u - x.base - TC_OVERHEAD;
-        if (u == x.base || block < tc_edge(c, x)) {
+        x.h = (u - x.base) / x.units();
+        x.base += x.h * x.units();
+        block = u > x.base + x.opening ? (u - x.base - x.opening) / x.per_block : 0;
+        if (block < tc_edge(c, x)) {
             block = 0;
         } else if (block > x.nb - tc_edge(c, x)) {
             tc_next(c, x);
@@ -684,24 +692,32 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
             }
         } else if (warp == 10) {
             // ------------------------------------------------------- units of every sequence, their running sum, the CTA's segments
-            const TcBatch g(a, sh.info);
+            TcBatch g(a, sh.info);
             const int seqs = a.B.n;
+            auto count = [&](int i) {   // units of sequence i
+                if (i >= seqs) return 0;
+                TcTile x;
+                x.s = g.seq(i);
+                int units = 0;
+#pragma unroll 1
+                for (x.t = 0; x.t * g.step < x.s.rows; ++x.t) {
+                    tc_span(g, x);
+                    units = min(units + x.units(), TC_MOST);
+                }
+                return (int)min((long long)units * a.P.kv, (long long)TC_MOST);
+            };
+            if (seqs <= 32) {   // (a small batch)
+                g.open = 0;
+                int units = count(lane);
+                for (int o = 16; o; o >>= 1) units = min(units + __shfl_xor_sync(~0u, units, o), TC_MOST);
+                if (units >= TC_FEW * p.n_ctas) g.open = TC_OPEN;
+            }
             int total = 0;
             if (lane == 0) sh.prefix[0] = 0;
 #pragma unroll 1
             for (int i0 = 0; i0 < seqs; i0 += 32) {   // a lane a sequence
                 const int i = i0 + lane;
-                int units = 0;
-                if (i < seqs) {
-                    TcTile x;
-                    x.s = g.seq(i);
-#pragma unroll 1
-                    for (x.t = 0; x.t * g.step < x.s.rows; ++x.t) {
-                        tc_span(g, x);
-                        units = min(units + x.nb + TC_OVERHEAD, TC_MOST);
-                    }
-                }
-                units = (int)min((long long)units * a.P.kv, (long long)TC_MOST);
+                int units = count(i);
                 if (seqs > 1)
                     for (int o = 1; o < 32; o <<= 1) {
                         const int y = __shfl_up_sync(~0u, units, o);
@@ -742,7 +758,9 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                     if (!more) break;
                     // the first of a cut tile's pieces says how many follow: the cuts that stay inside the tile
                     if (wk.j0 == 0 && wk.j1 < wk.x.nb) {
-                        const int edge = tc_edge(g, wk.x), lo = wk.x.base + TC_OVERHEAD + edge, hi = wk.x.base + TC_OVERHEAD + wk.x.nb - edge;
+                        // (block >= edge and block <= nb - edge, in units)
+                        const int edge = tc_edge(g, wk.x), from = wk.x.base + wk.x.opening;
+                        const int lo = from + edge * wk.x.per_block, hi = from + (wk.x.nb - edge + 1) * wk.x.per_block - 1;
                         int *mt = p.meta + cta * 8;
                         cuts = hi / per - (lo - 1) / per;
                         mt[1] = wk.x.s.first + wk.x.tok0; mt[2] = wk.x.ntok; mt[3] = wk.x.h; mt[4] = !F32 && wk.x.ntok > tq;
@@ -1082,7 +1100,7 @@ __device__ __noinline__ void attend_mend(const AttendParams &a, int t, int warp,
 // An infinity or NaN in V at a position that some rows of a tile do not see has met their weight of 0 in the product.  Such
 // rows show it by not being finite; they are done over here, position by position.
 template <int D, int TY>
-__global__ void __launch_bounds__(256, 4) attend_join_kernel(const __grid_constant__ TcParams p) {
+__global__ void __launch_bounds__(256, 3) attend_join_kernel(const __grid_constant__ TcParams p) {
     constexpr int LANES = D / 4, ROWS = 32 / LANES;   // lanes a row, four values each; rows a warp
     typedef typename Elem<TY>::T T;
     typedef typename Elem<TY == PTY_BF16 ? PTY_BF16 : PTY_F16>::T C;
@@ -1108,14 +1126,32 @@ __global__ void __launch_bounds__(256, 4) attend_join_kernel(const __grid_consta
             for (int i = ch; i <= more; i += LANES) top = fmaxf(top, p.ml[(long long)at(i) * 2]);
 #pragma unroll
             for (int x = LANES / 2; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-#pragma unroll 4
-            for (int i = 0; i <= more; ++i) {
-                const float2 ml = *(const float2 *)(p.ml + (long long)at(i) * 2);
-                const float4 v = *(const float4 *)(p.part + (long long)at(i) * D + ch * 4);
-                const float b = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-                l = fmaf(b, ml.y, l);
-                o.x = fmaf(b, v.x, o.x); o.y = fmaf(b, v.y, o.y); o.z = fmaf(b, v.z, o.z); o.w = fmaf(b, v.w, o.w);
+#pragma unroll 1
+            for (int i0 = 0; i0 <= more; i0 += LANES) {
+                float b = 0.f;   // the lane's piece: its weight
+                if (i0 + ch <= more) {
+                    const float2 ml = *(const float2 *)(p.ml + (long long)at(i0 + ch) * 2);
+                    if (ml.x != -INFINITY) b = ex2(ml.x - top);
+                    l = fmaf(b, ml.y, l);
+                }
+                const int n = min(LANES, more + 1 - i0);
+                const float *src = p.part + (long long)at(i0) * D + ch * 4;
+                const long long step = 2ll * p.ws_rows * D, jump = i0 == 0 ? step - (long long)p.ws_rows * D : step;   // (piece 0 lies in slot 1)
+#pragma unroll 1
+                for (int i = 0; i < n; i += 8) {   // eight pieces' loads at a time
+                    float4 v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (i + k < n) v[k] = *(const float4 *)(src + (i + k == 0 ? 0 : jump + (i + k - 1) * step));
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float bi = __shfl_sync(~0u, b, (sub * LANES) | ((i + k) & (LANES - 1)));
+                        if (i + k < n) { o.x = fmaf(bi, v[k].x, o.x); o.y = fmaf(bi, v[k].y, o.y); o.z = fmaf(bi, v[k].z, o.z); o.w = fmaf(bi, v[k].w, o.w); }
+                    }
+                }
             }
+#pragma unroll
+            for (int x = LANES / 2; x; x >>= 1) l += __shfl_xor_sync(~0u, l, x);
             const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
             o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
             const int row = row0 + tok, head = h * a.group + rr % a.group;
