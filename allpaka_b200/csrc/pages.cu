@@ -29,11 +29,13 @@ __device__ __forceinline__ void put(void *p, long long i, int ty, float x) {
 
 // Where a row of the batch belongs: its position in its sequence and where that is stored (-1: nowhere; -2: the row is nobody's).
 struct RopeAt { int pos, page; };
-constexpr int ROPE_MOST = 8;   // rows that a block takes
+constexpr int ROPE_MOST = 8;   // rows that a block takes at a time
 
 // The places and the sines and cosines of a block's rows, side by side: a warp looks for a row's sequence, 32 offsets at a time
 // instead of a chain of loads.  Angles: position * turns(pair) in 64 bits, whole turns taken off, then sine and cosine of the rest
-// in 32 bits: at a position of 2^20 a 32-bit product would already be 2^-4 radians off.
+// in 32 bits: at a position of 2^20 a 32-bit product would already be 2^-4 radians off.  Pair j lies at cs[rope_slot(j)]: the
+// threads of a head, which hold eight neighbouring pairs each, read 8-byte neighbours.
+__device__ __forceinline__ int rope_slot(int j) { return (j & 7) * 16 + (j >> 3); }
 __device__ __forceinline__ void rope_places(const RopeParams &p, int t0, int rows, RopeAt *at, int *turn_at, float2 *cs) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp < rows) {
@@ -57,7 +59,7 @@ __device__ __forceinline__ void rope_places(const RopeParams &p, int t0, int row
         const double a = (double)turn_at[row] * p.turn[j];
         float sn, cn;
         sincospif((float)(2.0 * (a - rint(a))), &sn, &cn);
-        cs[row * 128 + j] = make_float2(cn * p.mag, sn * p.mag);
+        cs[row * 128 + rope_slot(j)] = make_float2(cn * p.mag, sn * p.mag);
     }
     __syncthreads();
 }
@@ -116,83 +118,100 @@ __device__ __forceinline__ void store8(void *p, long long at, int ty, const floa
 
 // Heads of 16 * LANES dimensions, rotated in whole groups of 16: LANES threads a head, 16 values each (8 pairs, or 16 that pass
 // through), so that every access is 16 bytes wide.  Bound by the bytes; what stands in the way is latency: finding a row's place
-// and its angles is a chain of four loads and 64-bit arithmetic, about 2 us, so a block of a long batch takes eight rows, works
-// their places out together, and has its first loads under way before it begins.
+// and its angles is a chain of four loads and 64-bit arithmetic, about 2 us, so a block takes eight rows of its share at a time,
+// works their places out together, and has its first loads under way before it begins; three blocks share a multiprocessor.
 template <int TY, int LANES>
-__global__ void __launch_bounds__(256) rope_append_wide_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(256, 3) rope_append_wide_kernel(const __grid_constant__ RopeParams p) {
     typedef typename Elem<TY>::T T;
-    constexpr int AHEAD = TY == PTY_F32 ? 2 : 4, AT_ONCE = 256 / LANES;   // heads that the block works on side by side
+    constexpr int AHEAD = TY == PTY_F32 ? 1 : 2, AT_ONCE = 256 / LANES;   // heads that the block works on side by side
     __shared__ float2 cs[ROPE_MOST * 128];
     __shared__ RopeAt place[ROPE_MOST];
     __shared__ int turn_at[ROPE_MOST];
     pages_let_next();
     pages_wait_front();
-    const int t0 = blockIdx.x * p.rows_per_block, rows = min(p.rows_per_block, p.B.rows - t0);
-    const int u = threadIdx.x % LANES, heads = p.heads + 2 * p.P.kv, units = rows * heads;
+    const int u = threadIdx.x % LANES, heads = p.heads + 2 * p.P.kv;
     const bool turned = u < p.rot / 16;
     const int o0 = turned && !p.pairs ? u * 8 : u * 16, o1 = turned && !p.pairs ? p.rot / 2 + u * 8 : u * 16 + 8;
-    Raw16<TY> raw[AHEAD];
-    auto load = [&](int i0) {
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            const int i = i0 + a * AT_ONCE + threadIdx.x / LANES;
-            if (i >= units) break;
-            const int t = t0 + i / heads, r = i % heads;
-            const T *src = r < p.heads ? (const T *)p.q + t * p.qs[0] + r * p.qs[1]
-                           : r < p.heads + p.P.kv ? (const T *)p.k + t * p.ks[0] + (r - p.heads) * p.ks[1]
-                                                  : (const T *)p.v + t * p.vs[0] + (r - p.heads - p.P.kv) * p.vs[1];
-            load16<TY>(raw[a], src, o0, o1);
-        }
-    };
-    load(0);
-    rope_places(p, t0, rows, place, turn_at, cs);
     const int cache = p.P.bf16 ? PTY_BF16 : PTY_F16;
-    for (int i0 = 0; i0 < units; i0 += AHEAD * AT_ONCE) {
-        if (i0) load(i0);
+    const int end = (int)((long long)p.B.rows * (blockIdx.x + 1) / gridDim.x);
+    for (int t0 = (int)((long long)p.B.rows * blockIdx.x / gridDim.x); t0 < end; t0 += ROPE_MOST) {
+        const int rows = min(ROPE_MOST, end - t0);
+        // The thread's heads: (row, head) AT_ONCE heads on each time; one sequence of them to load, one to work on.
+        struct At { int row, r; };
+        auto on = [&](At &x) {
+            x.r += AT_ONCE;
+            while (x.r >= heads) { x.r -= heads; ++x.row; }
+        };
+        At next = {0, (int)(threadIdx.x / LANES) - AT_ONCE}, cur = next;
+        Raw16<TY> ping[AHEAD], pong[AHEAD];   // one is on its way while the other is worked on
+        auto load = [&](Raw16<TY> *raw) {
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            if (i0 + a * AT_ONCE >= units) break;   // (the whole block)
-            const int i = i0 + a * AT_ONCE + threadIdx.x / LANES, row = min(i / heads, rows - 1), r = i % heads;
-            float y[16];
-            widen16<TY>(raw[a], y);
-            const int kind = r < p.heads ? 0 : (r < p.heads + p.P.kv ? 1 : 2);
-            if (p.q_norm || p.k_norm) {
-                const float *w = kind == 0 ? p.q_norm : (kind == 1 ? p.k_norm : nullptr);
-                float ss = 0.f;
+            for (int a = 0; a < AHEAD; ++a) {
+                on(next);
+                if (next.row >= rows) continue;
+                const int t = t0 + next.row, r = next.r;
+                const T *src = r < p.heads ? (const T *)p.q + t * p.qs[0] + r * p.qs[1]
+                               : r < p.heads + p.P.kv ? (const T *)p.k + t * p.ks[0] + (r - p.heads) * p.ks[1]
+                                                      : (const T *)p.v + t * p.vs[0] + (r - p.heads - p.P.kv) * p.vs[1];
+                load16<TY>(raw[a], src, o0, o1);
+            }
+        };
+        auto work = [&](const Raw16<TY> *raw, int i0) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) ss = fmaf(y[e], y[e], ss);
+            for (int a = 0; a < AHEAD; ++a) {
+                if (i0 + a * AT_ONCE >= rows * heads) break;   // (the whole block)
+                on(cur);
+                const int row = min(cur.row, rows - 1), r = cur.r;
+                float y[16];
+                widen16<TY>(raw[a], y);
+                const int kind = r < p.heads ? 0 : (r < p.heads + p.P.kv ? 1 : 2);
+                if (p.q_norm || p.k_norm) {
+                    const float *w = kind == 0 ? p.q_norm : (kind == 1 ? p.k_norm : nullptr);
+                    float ss = 0.f;
 #pragma unroll
-                for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
-                if (w) {
-                    const float rs = rsqrtf(ss / (float)p.P.dim + p.eps);
+                    for (int e = 0; e < 16; ++e) ss = fmaf(y[e], y[e], ss);
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const float4 g = __ldg((const float4 *)(w + (e < 8 ? o0 + e : o1 + e - 8)));
-                        y[e] *= rs * g.x; y[e + 1] *= rs * g.y; y[e + 2] *= rs * g.z; y[e + 3] *= rs * g.w;
+                    for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+                    if (w) {
+                        const float rs = rsqrtf(ss / (float)p.P.dim + p.eps);
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            const float4 g = __ldg((const float4 *)(w + (e < 8 ? o0 + e : o1 + e - 8)));
+                            y[e] *= rs * g.x; y[e + 1] *= rs * g.y; y[e + 2] *= rs * g.z; y[e + 3] *= rs * g.w;
+                        }
                     }
                 }
-            }
-            if (kind < 2 && turned) {
-                const float2 *z = cs + row * 128 + u * 8;
-                if (p.pairs) {
+                if (kind < 2 && turned) {
+                    const float2 *z = cs + row * 128 + u;
+                    if (p.pairs) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) rope_turn(y[2 * e], y[2 * e + 1], z[e]);
-                } else {
+                        for (int e = 0; e < 8; ++e) rope_turn(y[2 * e], y[2 * e + 1], z[16 * e]);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) rope_turn(y[e], y[8 + e], z[e]);
+                        for (int e = 0; e < 8; ++e) rope_turn(y[e], y[8 + e], z[16 * e]);
+                    }
                 }
+                const RopeAt at = place[row];
+                if (cur.row >= rows || at.page == -2 || (kind && at.page < 0)) continue;
+                const long long t = t0 + row, in = at.pos & (p.P.page - 1);
+                void *dst = p.out;
+                long long to = t * p.os[0] + r * p.os[1];
+                if (kind == 1) { dst = p.P.k; to = p.layer * p.P.ks[0] + at.page * p.P.ks[1] + in * p.P.ks[2] + (r - p.heads) * p.P.ks[3]; }
+                if (kind == 2) { dst = p.P.v; to = p.layer * p.P.vs[0] + at.page * p.P.vs[1] + in * p.P.vs[2] + (r - p.heads - p.P.kv) * p.P.vs[3]; }
+                const int ty = kind ? cache : p.out_ty;
+                store8(dst, to + o0, ty, y);
+                store8(dst, to + o1, ty, y + 8);
             }
-            const RopeAt at = place[row];
-            if (i >= units || at.page == -2 || (kind && at.page < 0)) continue;
-            const long long t = t0 + row, in = at.pos & (p.P.page - 1);
-            void *dst = p.out;
-            long long to = t * p.os[0] + r * p.os[1];
-            if (kind == 1) { dst = p.P.k; to = p.layer * p.P.ks[0] + at.page * p.P.ks[1] + in * p.P.ks[2] + (r - p.heads) * p.P.ks[3]; }
-            if (kind == 2) { dst = p.P.v; to = p.layer * p.P.vs[0] + at.page * p.P.vs[1] + in * p.P.vs[2] + (r - p.heads - p.P.kv) * p.P.vs[3]; }
-            const int ty = kind ? cache : p.out_ty;
-            store8(dst, to + o0, ty, y);
-            store8(dst, to + o1, ty, y + 8);
+        };
+        load(ping);
+        rope_places(p, t0, rows, place, turn_at, cs);
+        for (int i0 = 0; i0 < rows * heads; i0 += 2 * AHEAD * AT_ONCE) {
+            load(pong);
+            work(ping, i0);
+            load(ping);
+            work(pong, i0 + AHEAD * AT_ONCE);
         }
+        __syncthreads();   // (the places and angles are read until here)
     }
 }
 
@@ -250,8 +269,9 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
             const int da = p.pairs ? 2 * j : j, db = p.pairs ? 2 * j + 1 : j + half;
             float a = to_f32(src[da]), b = to_f32(src[db]);
             if (w) { a = a * rs * w[da]; b = b * rs * w[db]; }
-            put(dst, at + da, ty, a * cs[j].x - b * cs[j].y);
-            put(dst, at + db, ty, b * cs[j].x + a * cs[j].y);
+            const float2 z = cs[rope_slot(j)];
+            put(dst, at + da, ty, a * z.x - b * z.y);
+            put(dst, at + db, ty, b * z.x + a * z.y);
         }
         for (int d = p.rot + lane; d < D; d += 32) {
             float x = to_f32(src[d]);
@@ -508,13 +528,11 @@ unsigned copy_blocks(const PagesDev &P, long long n, int n_sm) {
 }  // namespace
 
 template <int TY>
-cudaError_t launch_rope(RopeParams p, int n_sm, cudaStream_t st) {
+cudaError_t launch_rope(const RopeParams &p, int n_sm, cudaStream_t st) {
     // weights are read 16 bytes at a time; their start is the caller's
     const bool weights = (((uintptr_t)p.q_norm | (uintptr_t)p.k_norm) & 15) == 0;
     if (p.rot % 16 == 0 && weights && (p.P.dim == 64 || p.P.dim == 128 || p.P.dim == 256)) {
-        // one row a block while that fills the multiprocessors twice over, up to eight as the batch grows
-        p.rows_per_block = std::max(1, std::min(ROPE_MOST, p.B.rows / (2 * n_sm)));
-        const dim3 grid((p.B.rows + p.rows_per_block - 1) / p.rows_per_block);
+        const dim3 grid(std::min(p.B.rows, 3 * n_sm));
         if (p.P.dim == 64) return launch_front(rope_append_wide_kernel<TY, 4>, grid, 256, 0, st, p);
         if (p.P.dim == 128) return launch_front(rope_append_wide_kernel<TY, 8>, grid, 256, 0, st, p);
         return launch_front(rope_append_wide_kernel<TY, 16>, grid, 256, 0, st, p);

@@ -106,7 +106,6 @@ struct RopeParams {
     const int *positions;        // per row, or null: the row's own position in its sequence
     const float *q_norm, *k_norm;
     float eps;
-    int rows_per_block;          // (the launch's)
     int rot, pairs;              // dimensions rotated; 1: neighbouring pairs, 0: halves
     float mag;                   // factor on sine and cosine
     double turn[128];            // turns a position, per pair
