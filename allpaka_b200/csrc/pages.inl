@@ -158,8 +158,11 @@ int rope_frequencies(const char *what, const apk_rope *r, uint32_t dim, RopePara
         hi = std::min(std::ceil(pair(r->beta_slow)), rot - 1.0);
         if (factor > 1.0) mag *= 0.1 * std::log(factor) + 1.0;
     }
-    for (int i = 0; i < half; ++i) {
-        double f = std::pow(base, -2.0 * i / rot);
+    // one power, then products: 128 of them are off by 2^-46 at most, 1e-8 of a turn at position 2^20
+    const double ratio = std::pow(base, -2.0 / rot);
+    double power = 1.0;
+    for (int i = 0; i < half; ++i, power *= ratio) {
+        double f = power;
         if (r->freq_factors) {
             if (!(r->freq_factors[i] > 0.f)) return fail(APK_ERR_INVALID_ARG, "%s: frequency factor %d is %g", what, i, r->freq_factors[i]);
             f /= r->freq_factors[i];
