@@ -104,7 +104,7 @@ __device__ __noinline__ void attend_row(const AttendParams &p, const SeqRows &s,
 // in 32 bits, while group 0 does the softmax of every block (tiles are narrow, two score and two O buffers).
 
 constexpr int TC_THREADS = 384;      // warps 0-7 softmax, 8 copies, 9 tensor instructions, 10 walks the segments, 11 completes the third register group
-constexpr int TC_STAGES = 4;
+constexpr int TC_MOST_STAGES = 8;     // blocks of K or V in the ring: 512 / D, 128 KB
 constexpr int TC_BLOCK = 128;         // positions a block
 // Units of work: a block of a narrow tile is one, of a wide tile two; opening and closing a tile costs as much as TC_OPEN blocks of
 // its own.   (64 sessions of 200 to 8192 positions: 122 us with 2, 116 with 3, 109 with 4, 110 with 6; a 4096-row chunk 454, 454, 447, 443.)
@@ -183,8 +183,8 @@ __host__ __device__ __forceinline__ void tc_next(const TcBatch &c, TcTile &x) {
 }
 
 // Fewest blocks of a piece of a cut tile: its rows are loaded, stored and joined once more, which costs a narrow tile about one
-// block's time and a wide one (up to 256 rows of partial sums) three.
-__host__ __device__ __forceinline__ int tc_edge(const TcBatch &c, const TcTile &x) { return x.ntok > c.tq ? 4 : 2; }
+// block's time and a wide one (up to 256 rows of partial sums) several.  (Mixed chunks 39 us with 4 for wide ones, 37 with 6 or 8.)
+__host__ __device__ __forceinline__ int tc_edge(const TcBatch &c, const TcTile &x) { return x.ntok > c.tq ? 6 : 2; }
 
 // Where the cut before unit u falls: a tile and a block of it (returned).  A cut too near to a tile's edge moves there.
 __host__ __device__ inline int tc_cut(const TcBatch &c, const int *prefix, int total, int u, TcTile &x) {
@@ -252,7 +252,7 @@ struct TcSegment {
 };
 
 struct TcShared {
-    uint64_t full[TC_STAGES], empty[TC_STAGES], seg_full[TC_SEGS], seg_empty[TC_SEGS], q_full, s_full[2], p_full[2], o_full[2], o_free[2], both, half, drain;
+    uint64_t full[TC_MOST_STAGES], empty[TC_MOST_STAGES], seg_full[TC_SEGS], seg_empty[TC_SEGS], q_full, s_full[2], p_full[2], o_full[2], o_free[2], both, half, drain;
     uint32_t tmem;
     int dead, odd;          // a wait ran out; a result is not finite
     int gone[2][8];         // per warp: a page of the segment is not there
@@ -524,18 +524,19 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
     constexpr bool BF = TY == PTY_BF16, F32 = TY == PTY_F32;
     constexpr int PARTS = F32 ? 2 : 1;
     constexpr uint32_t TILE = TC_BLOCK * D * 2;    // bytes of a Q tile or of a block of K or V
+    constexpr int STAGES = 512 / D;
     constexpr uint32_t O_COL = 256;                // TMEM columns: S0 S1 O0 O1
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t *const qs = smem, *const ring = smem + 2 * TILE;
-    TcShared &sh = *(TcShared *)(ring + TC_STAGES * TILE);
+    TcShared &sh = *(TcShared *)(ring + STAGES * TILE);
     const AttendParams &a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int tq = 128 / a.group;
 
     pages_let_next();   // (attend_join_kernel waits for this grid's end)
     if (tid == 0) {
-        for (int i = 0; i < TC_STAGES; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
         for (int i = 0; i < TC_SEGS; ++i) { mbar_init(&sh.seg_full[i], 1); mbar_init(&sh.seg_empty[i], 10); }
         for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 4); mbar_init(&sh.o_full[i], 1); mbar_init(&sh.o_free[i], 4); }
         mbar_init(&sh.q_full, 8);
@@ -590,7 +591,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                     else if (e == 2 * n - 1) { is_v = true; j = n - 1; }
                     else { is_v = !(e & 1); j = is_v ? (e - 2) >> 1 : (e + 1) >> 1; }
                     const int pos = (x.first + j) * TC_BLOCK;
-                    const int idx = ring0 + e, st = idx % TC_STAGES;
+                    const int idx = ring0 + e, st = idx % STAGES;
                     int pg = 0;
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv)
@@ -603,7 +604,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                             }
                             pg = __shfl_sync(~0u, pages[kv], ((j - from[kv]) << box_shift) + min(box, boxes - 1));
                         }
-                    ok = __all_sync(~0u, tc_wait(sh, &sh.empty[st], ((idx / TC_STAGES) & 1) ^ 1, p, 1));
+                    ok = __all_sync(~0u, tc_wait(sh, &sh.empty[st], ((idx / STAGES) & 1) ^ 1, p, 1));
                     if (!ok) break;
                     filled = idx + 1;
                     uint8_t *dst = ring + st * TILE;
@@ -620,8 +621,8 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                 ++n_seg;
             }
             // every copy that was asked for has arrived before the block ends
-            for (int idx = max(0, filled - TC_STAGES); idx < filled; ++idx)
-                (void)mbar_wait_bounded(&sh.full[idx % TC_STAGES], (idx / TC_STAGES) & 1, p.wait_limit);
+            for (int idx = max(0, filled - STAGES); idx < filled; ++idx)
+                (void)mbar_wait_bounded(&sh.full[idx % STAGES], (idx / STAGES) & 1, p.wait_limit);
         } else if (warp == 9) {
             // -------------------------------------------------------- tensor instructions: issued by one thread of a warp that stays
             // together, so that their operands are the warp's and not the thread's (one thread alone took 85 cycles for each)
@@ -646,8 +647,8 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                     const int w = i & 1;
                     const bool last = i + 2 >= steps, both = !wide || w;   // both: no other group needs the block any more
                     if (i >= 0) {
-                        const int v = ring0 + tc_slot_v(wide, wide ? i >> 1 : i, n), st = v % TC_STAGES;
-                        if (!(ok = __all_sync(~0u, tc_wait(sh, &sh.full[st], (v / TC_STAGES) & 1, p, 2) && tc_wait(sh, &sh.p_full[w], ph_p >> w & 1, p, 3)))) break;
+                        const int v = ring0 + tc_slot_v(wide, wide ? i >> 1 : i, n), st = v % STAGES;
+                        if (!(ok = __all_sync(~0u, tc_wait(sh, &sh.full[st], (v / STAGES) & 1, p, 2) && tc_wait(sh, &sh.p_full[w], ph_p >> w & 1, p, 3)))) break;
                         ph_p ^= 1u << w;
                         tc_fence_after();
                         if (leader) {
@@ -664,8 +665,8 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                         }
                     }
                     if (!last) {
-                        const int kn = ring0 + tc_slot_k(wide, wide ? (i + 2) >> 1 : i + 2), st = kn % TC_STAGES;
-                        if (!(ok = __all_sync(~0u, tc_wait(sh, &sh.full[st], (kn / TC_STAGES) & 1, p, 2)))) break;
+                        const int kn = ring0 + tc_slot_k(wide, wide ? (i + 2) >> 1 : i + 2), st = kn % STAGES;
+                        if (!(ok = __all_sync(~0u, tc_wait(sh, &sh.full[st], (kn / STAGES) & 1, p, 2)))) break;
                         tc_fence_after();
                         if (leader) {
                             const uint64_t qa = tc_desc(q_addr + (wide ? w * TILE : 0), 16), ka = tc_desc(r_addr + st * TILE, 16);
@@ -888,9 +889,9 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
             // What lies behind the sequence in its last page takes part in the product with weight 0: it may not be NaN.
             auto clear_tail = [&](int j, int pos) {
                 const int idx = ring0 + tc_slot_v(wide, j, n);
-                if (!wait(&sh.full[idx % TC_STAGES], (idx / TC_STAGES) & 1, 6)) return false;
+                if (!wait(&sh.full[idx % STAGES], (idx / STAGES) & 1, 6)) return false;
                 if (pos + r >= x.s.len) {
-                    uint8_t *v = ring + (idx % TC_STAGES) * TILE + r * 128;
+                    uint8_t *v = ring + (idx % STAGES) * TILE + r * 128;
 #pragma unroll
                     for (int k = 0; k < PANELS * 8; ++k) *(uint4 *)(v + (k >> 3) * (TC_BLOCK * 128) + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
                 }
@@ -1207,7 +1208,7 @@ TcSize tc_size(const AttendParams &p, int n_sm) {
 
 template <int D>
 constexpr int tc_smem() {
-    constexpr int n = 1024 + (2 + TC_STAGES) * TC_BLOCK * D * 2 + (int)sizeof(TcShared) + 4 * PAGES_MAX_BATCH;
+    constexpr int n = 1024 + (2 + 512 / D) * TC_BLOCK * D * 2 + (int)sizeof(TcShared) + 4 * PAGES_MAX_BATCH;
     static_assert(n <= 232448, "shared memory of a block");
     return n;
 }
