@@ -114,6 +114,7 @@ constexpr int TC_FEW = 4;             // fewer units a CTA than this, without th
 constexpr int TC_MOST = 1 << 30;      // units of a call (the host has bounded a proper batch's)
 constexpr int TC_SEGS = 4;            // segments that are known ahead
 constexpr int TC_INFO = 256;          // sequences that a block keeps a copy of
+constexpr long long TC_DRAIN = 1ll << 31;  // cycles that a block waits for its own copies and products at its end, whatever the waits' budget
 constexpr float TC_LAZY = 8.f;
 
 struct TcParams {
@@ -622,7 +623,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
             }
             // every copy that was asked for has arrived before the block ends
             for (int idx = max(0, filled - STAGES); idx < filled; ++idx)
-                (void)mbar_wait_bounded(&sh.full[idx % STAGES], (idx / STAGES) & 1, p.wait_limit);
+                (void)mbar_wait_bounded(&sh.full[idx % STAGES], (idx / STAGES) & 1, TC_DRAIN);
         } else if (warp == 9) {
             // -------------------------------------------------------- tensor instructions: issued by one thread of a warp that stays
             // together, so that their operands are the warp's and not the thread's (one thread alone took 85 cycles for each)
@@ -689,7 +690,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
             }
             if (leader) {
                 tc_commit(&sh.drain);
-                (void)mbar_wait_bounded(&sh.drain, 0, p.wait_limit);
+                (void)mbar_wait_bounded(&sh.drain, 0, TC_DRAIN);
             }
         } else if (warp == 10) {
             // ------------------------------------------------------- units of every sequence, their running sum, the CTA's segments

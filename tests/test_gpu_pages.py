@@ -172,6 +172,91 @@ def test_attention_scores_far_from_zero(G, g):
             attend_case(G, g, [1, 60], [700, 400], rows_ty=ty, spoil=spoil, scale=scale)
 
 
+@pytest.mark.parametrize("cache,rows_ty", KINDS)
+def test_attention_many_sequences(G, g, cache, rows_ty):
+    """More sequences than a block keeps a copy of, single tokens and small chunks, empty ones among them."""
+    rnd = random.Random(12)
+    rows = [rnd.choice([0, 1, 1, 1, 2, 5]) for _ in range(700)]
+    lens = [max(r, rnd.choice([0, 1, 17, 130, 400])) for r in rows]
+    attend_case(G, g, rows, lens, cache=cache, rows_ty=rows_ty, kv=1, group=4, dim=64, page=32)
+
+
+@pytest.mark.parametrize("dim,group,cache", [(128, 4, "f16"), (64, 8, "bf16"), (128, 5, "bf16")])
+def test_attention_long_chunks_and_long_sequences(G, g, dim, group, cache):
+    """Tiles that are cut over many blocks of the grid: a chunk of a thousand rows, and one row over twenty thousand positions."""
+    attend_case(G, g, [1000, 1, 33], [1500, 20000, 5000], cache=cache, kv=1, group=group, dim=dim, page=128)
+
+
+def test_attention_long_sequence_of_32_bit_rows(G, g):
+    attend_case(G, g, [8, 1], [9000, 12345], rows_ty="f32", kv=2, group=5, page=16)
+
+
+def test_attention_of_rows_past_32_bit_offsets(G, g):
+    """The pages of the sequence lie behind more than 2^31 elements of the pool."""
+    n_pages, page, kv, dim = 140000, 16, 8, 128
+    pool = Pool(1, 1, page, kv, dim, "f16", 2, 8)
+    pool.k = torch.empty((1, n_pages, page, kv, dim), dtype=torch.float16, device="cuda")
+    pool.v = torch.empty((1, n_pages, page, kv, dim), dtype=torch.float16, device="cuda")
+    assert pool.k.numel() > 2 ** 31
+    pool.refs = torch.zeros(n_pages, dtype=torch.int32, device="cuda")
+    pool.free = list(range(n_pages - 20, n_pages))
+    r = gen(40)
+    k, v = pool.fill(1, 100, r)
+    pages = G.KvPages(g, *pool.args())
+    q = torch.randn((3, 16, dim), generator=r, device="cuda").half()
+    out = torch.empty_like(q)
+    new = [torch.randn((3, h, dim), generator=r, device="cuda").half() for h in (16, kv, kv)]
+    assert g.rope_append(pages, 0, *new, ints([0, 3]), None, out=out, seqs=ints([1]), wait=True)
+    assert torch.equal(pool.read(1)[0][97:], new[1]) and torch.equal(pool.read(1)[1][97:], new[2])
+    k, v = pool.read(1)
+    assert g.attend_pages(pages, 0, q, ints([0, 3]), 0.1, out, seqs=ints([1]), wait=True)
+    ref = attend64(q, k, v, 0.1)
+    assert float(((out.double() - ref[0]).abs() - attend_bound(*ref, "f16")).max()) <= 0
+    # a fork far up there, copied to the pool's front
+    assert g.pages_fork(pages, [1], [0]) and g.pages_reserve(pages, [0], [1])
+    assert int(pool.table[0, 6]) == 0 and torch.equal(pool.k[0, 0, :4], k[96:])
+
+
+def test_attention_workspaces(G, g):
+    """A workspace of the caller's own; too small a one is refused; two calls at once on two streams each have theirs."""
+    pool = Pool(1, 700, 16, 2, 128, "f16", 2, 600, seed=50)
+    r = gen(50)
+    held = [pool.fill(0, 5000, r), pool.fill(1, 3000, r)]
+    pages = G.KvPages(g, *pool.args())
+    qs = [torch.randn((1, 8, 128), generator=r, device="cuda").half() for _ in range(2)]
+    outs, cu = [torch.empty_like(q) for q in qs], ints([0, 1])
+    seqs = [ints([0]), ints([1])]
+    with pytest.raises(G.GpuError) as e:
+        g.attend_pages(pages, 0, qs[0], cu, 0.1, outs[0], workspace=torch.empty(100, dtype=torch.uint8, device="cuda"))
+    assert e.value.code == -1
+    own = torch.empty(40 << 20, dtype=torch.uint8, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(2):   # handed a stream that is not the current one
+            assert g.attend_pages(pages, 0, qs[i], cu, 0.1, outs[i], seqs=seqs[i], stream=streams[i].cuda_stream, workspace=own if i else None)
+    torch.cuda.synchronize()
+    for i in range(2):
+        ref = attend64(qs[i], *held[i], 0.1)
+        assert float(((outs[i].double() - ref[0]).abs() - attend_bound(*ref, "f16")).max()) <= 0
+
+
+def test_attention_is_repeatable(G, g):
+    """The same call gives the same bits: nothing depends on the order in which blocks come."""
+    pool = Pool(1, 900, 16, 4, 128, "bf16", 3, 500, seed=51)
+    r = gen(51)
+    for s, l in enumerate((6000, 17, 2500)):
+        pool.fill(s, l, r)
+    pages = G.KvPages(g, *pool.args())
+    q = torch.randn((302, 16, 128), generator=r, device="cuda").bfloat16()
+    got = []
+    for _ in range(5):
+        out = torch.empty_like(q)
+        assert g.attend_pages(pages, 0, q, ints([0, 1, 2, 302]), 0.09, out, wait=True)
+        got.append(out)
+    assert all(torch.equal(got[0], x) for x in got[1:])
+
+
 def test_attention_agrees_with_the_contiguous_cache(G, g):
     """The same keys and values in an apk_kv and in pages: 32-bit rows, one and eight of them."""
     kv, dim, length = 4, 128, 777
