@@ -88,9 +88,9 @@ __device__ __noinline__ void attend_row(const AttendParams &p, const SeqRows &s,
 // attend_join_kernel merges in a fixed order.
 //
 // Two groups of four warps for the softmax (thread = row = TMEM lane), a warp that walks the CTA's range and hands out its
-// segments, one that issues TMA copies, one that issues the tensor instructions.  S = Q K^T (both from shared memory) goes to TMEM; the softmax group turns its 128 x 128
-// scores into 16-bit weights P over the same TMEM columns; O += P V takes P from TMEM and V from shared memory
-// (transposed by its descriptor).
+// segments, one that issues TMA copies, one that issues the tensor instructions.  S = Q K^T (both from shared memory) goes
+// to TMEM; the softmax group turns its 128 x 128 scores into 16-bit weights P over the same TMEM columns; O += P V takes P
+// from TMEM and V from shared memory (transposed by its descriptor).
 //   wide tile (more than 128 rows): group w works on rows 128w.. and shares every K and V block with the other;
 //   narrow tile (one token of a few heads, mostly): both groups hold the same rows, group w takes every second block,
 //   and group 0 joins the two results, which lie on the same TMEM lanes.  Up to 32 rows lie in TMEM four times, and each
@@ -102,12 +102,20 @@ __device__ __noinline__ void attend_row(const AttendParams &p, const SeqRows &s,
 // values, 22 bits; every product is done for both.  The tensor cores' sums are truncated at about 24 bits, and over the
 // blocks of a long sequence that would add up to 2^-15: so O of a block starts from 0, and group 1 adds it to its registers
 // in 32 bits, while group 0 does the softmax of every block (tiles are narrow, two score and two O buffers).
+//
+// What bounds it, and what it measured.  Single tokens: the bytes of K and V; 64 sessions of 200 to 8192 positions (577 MB)
+// 107 us, 5.4 TB/s or 0.84 of the measured copy rate; one of 131077 positions 97 us, 0.86; the rest is 15 us of opening,
+// joining and cold code.  Chunks: a group's chain scores -> weights (1.1 us for 128 x 128: the exponentials alone are 0.6) ->
+// both products (0.6) -> scores, with 0.5 us of hand-overs in between; two groups in turn keep the tensor cores half busy:
+// 4096 rows over 8192 positions 447 us, 920 TFLOP/s.  TMEM is full (two times 128 columns of scores and of O), so there is
+// no third group and no second score buffer; 64-position steps with two of them took 600 us.
+// 32-bit rows: the tensor cores' time for every product done twice, 1.7 us a block.
 
 constexpr int TC_THREADS = 384;      // warps 0-7 softmax, 8 copies, 9 tensor instructions, 10 walks the segments, 11 completes the third register group
 constexpr int TC_MOST_STAGES = 8;     // blocks of K or V in the ring: 512 / D, 128 KB
 constexpr int TC_BLOCK = 128;         // positions a block
 // Units of work: a block of a narrow tile is one, of a wide tile two; opening and closing a tile costs as much as TC_OPEN blocks of
-// its own.   (64 sessions of 200 to 8192 positions: 122 us with 2, 116 with 3, 109 with 4, 110 with 6; a 4096-row chunk 454, 454, 447, 443.)
+// its own.  (64 sessions of 200 to 8192 positions: 122 us with 2, 116 with 3, 109 with 4, 110 with 6; a 4096-row chunk 454, 454, 447, 443.)
 constexpr int TC_OPEN = 4;
 constexpr int TC_MIN_UNITS = 2;       // least range of a CTA
 constexpr int TC_FEW = 4;             // fewer units a CTA than this, without the opening: it is not counted, so that all CTAs have a share
@@ -270,7 +278,7 @@ struct TcShared {
 __host__ __device__ __forceinline__ int tc_slot_k(bool wide, int j) { return wide ? 2 * j : (j < 2 ? j : 2 * j - 1); }
 __host__ __device__ __forceinline__ int tc_slot_v(bool wide, int j, int n) { return wide ? 2 * j + 1 : (j < n - 1 ? 2 * j + 2 : 2 * n - 1); }
 
-// (out of line, like all that a block of scores does not need: the code of a block's loop and its registers are what counts)
+// A bounded wait; the first to run out is recorded, and nobody else waits for long after it.
 __device__ __forceinline__ bool tc_wait_on(TcShared &sh, uint64_t *bar, uint32_t parity, int *err, long long limit, int site) {
     if (*(volatile int *)&sh.dead) return false;
     if (mbar_wait_bounded(bar, parity, limit)) return true;

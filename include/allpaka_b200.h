@@ -408,16 +408,17 @@ void apk_stats(apk_ctx *ctx, apk_stats_t *out);
  *     apk_rope_append, apk_attend_pages           per layer
  *     apk_pages_fork / _release / _compact        between steps, as sequences branch and end
  *
- * All memory is the caller's DEVICE memory and all work goes to the caller's stream, in its order; no
- * call allocates or synchronises (but with wait != 0), so each can be captured into a CUDA graph: the
- * lengths, the page table and the batch are read by the kernels, the lists of _reserve, _fork and
- * _release are part of the captured launch.  Calls that change one pool (and calls that read it
- * meanwhile) are ordered by the caller; calls on different pools are independent of one another.
+ * All memory is the caller's DEVICE memory, on the context's device, and all work goes to the caller's
+ * stream, in its order; no call allocates or synchronises (but with wait != 0, which a capture cannot
+ * have), so each can be captured into a CUDA graph: the lengths, the page table and the batch are read
+ * by the kernels, the lists of _reserve, _fork and _release are part of the captured launch.  Calls
+ * that change one pool (and calls that read it meanwhile) are ordered by the caller; calls on different
+ * pools are independent of one another.  The caller's current device is left as it was.
  *
  * Nothing that the device arrays hold can lead outside the buffers: a page number outside the pool is
  * a page that is not there (its positions are not visible, stores to it are dropped), a length is cut
  * to the row of the table, a sequence number outside the table has no positions, row offsets are cut to
- * n_rows. */
+ * n_rows (they rise; what rows get that several sequences claim is not defined). */
 #define APK_PAGES_MAX_LIST 1024u  /* sequences one _reserve, _fork or _release names */
 #define APK_PAGES_MAX_BATCH 4096u /* sequences of one _rope_append or _attend */
 /* int32 values of apk_pages.work, the pool's scratch: zeroed by the caller once, then left alone */
@@ -528,7 +529,8 @@ typedef struct {
 } apk_attend_req;
 /* The scratch a request needs (its pointers are not read); 0 for one that would be refused. */
 size_t apk_attend_pages_ws(apk_ctx *ctx, const apk_attend_req *req);
-/* wait != 0: synchronises the stream and reports an expired device-side wait. */
+/* wait != 0: synchronises the stream and reports an expired device-side wait (APK_ERR_TIMEOUT; one of
+ * an earlier call that was not waited for is reported by the next one on the pool that is). */
 int apk_attend_pages(apk_ctx *ctx, const apk_attend_req *req, void *stream, int wait);
 
 /* Human-readable reason for the last non-zero status on this thread
