@@ -259,7 +259,7 @@ int attend_view(const apk_attend_req *r, AttendParams *q) {
     p.causal = r->causal != 0;
     p.window = (int)r->window;
     // the kernels count (kv head, tile of rows, 128 positions) in 32 bits
-    const uint64_t tiles = (uint64_t)r->n_rows / (2u * (128u / (uint32_t)p.group)) + r->n;
+    const uint64_t tiles = (uint64_t)r->n_rows / (128u / (uint32_t)p.group) + r->n;
     if (tiles * (2 * ((uint64_t)r->pages->width * r->pages->page / 128 + 1) + 8) * kv >= (1ull << 30))
         return fail(APK_DECLINE_UNSUPPORTED_SHAPE, "%s: %u rows of %u sequences over tables of %u pages are too much for one call", what, r->n_rows, r->n, r->pages->width);
     return APK_OK;

@@ -573,6 +573,39 @@ def test_a_captured_step_is_replayed(G, g):
             assert float(((out[s:s + 1].double() - ref[0]).abs() - attend_bound(*ref, "f16")).max()) <= 0
 
 
+def test_captured_upkeep_is_replayed(G, g):
+    """Fork, growth, release and compaction in one CUDA graph: its lists stay, the state moves on with every replay."""
+    pool = Pool(2, 60, 8, 1, 64, "f16", 5, 12, seed=23)
+    pages, book = G.KvPages(g, *pool.args()), Book(60, 8, 5, 12)
+    assert g.pages_reserve(pages, [0, 1, 3], [13, 30, 5]) and book.reserve([0, 1, 3], [13, 30, 5])[0] == 0
+    page_map = torch.zeros(60, dtype=torch.int32, device="cuda")
+
+    def step():
+        assert g.pages_fork(pages, [0, 1], [2, 4])
+        assert g.pages_reserve(pages, [0, 2, 4], [3, 1, 9], wait=False)
+        assert g.pages_release(pages, [1, 3], [21, 2])
+        assert g.pages_compact(pages, page_map=page_map)
+
+    def by_hand():
+        book.fork([0, 1], [2, 4])
+        assert book.reserve([0, 2, 4], [3, 1, 9])[0] == 0
+        book.release([1, 3], [21, 2])
+        return book.compact()[0]
+
+    step()
+    by_hand()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(6):
+        graph.replay()
+        to = by_hand()
+        torch.cuda.synchronize()
+        same(pool, book)
+        assert page_map.tolist() == to and int(pages.short_by) == 0
+
+
 def test_streams_and_counters(G, g):
     """Work goes to the stream it is given (here: after a producer on that stream) and is counted."""
     pool = Pool(1, 40, 16, 2, 128, "f16", 1, 40, seed=31)
