@@ -773,7 +773,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                         const int lo = from + edge * wk.x.per_block, hi = from + (wk.x.nb - edge + 1) * wk.x.per_block - 1;
                         int *mt = p.meta + cta * 8;
                         cuts = hi / per - (lo - 1) / per;
-                        mt[1] = wk.x.s.first + wk.x.tok0; mt[2] = wk.x.ntok; mt[3] = wk.x.h; mt[4] = !F32 && wk.x.ntok > tq;
+                        mt[1] = wk.x.s.first + wk.x.tok0; mt[2] = wk.x.ntok; mt[3] = wk.x.h;
                     }
                     ++n_seg;
                     more = wk.next(g);
@@ -1090,25 +1090,41 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
     }
 }
 
-// The heads of row t whose results are not finite, done over position by position.
+// Row t's head hd over again, position by position.  The warp that calls it is the last to have stored the row.
 template <int D, typename T, typename C>
-__device__ __noinline__ void attend_mend(const AttendParams &a, int t, int warp, int lane) {
-    constexpr int E = D / 32;
+__device__ __noinline__ void attend_mend(const AttendParams &a, int t, int hd, int lane) {
     const int i = batch_find(a.B, t);
     if (i < 0) return;
     const SeqRows s = batch_seq(a.P, a.B, i);
+    __syncwarp();
+    attend_row<D, T, C>(a, s, t, hd, lane);
+}
+
+// The heads of row t that whole tiles have left not finite.  Rows of cut tiles are being stored by this very grid: who joins
+// them mends them.
+template <int D, typename T, typename C>
+__device__ __noinline__ void attend_mend_whole(const TcParams &p, int t, int warp, int lane) {
+    constexpr int E = D / 32;
+    const AttendParams &a = p.a;
     for (int hd = warp; hd < a.heads; hd += 8) {
+        bool cut = false;
+        for (int c = lane; c < p.n_ctas; c += 32) {
+            const int4 mt = *(const int4 *)(p.meta + c * 8);
+            cut |= mt.x > 0 && t >= mt.y && t < mt.y + mt.z && mt.w == hd / a.group;
+        }
+        if (__any_sync(~0u, cut)) continue;
         const T *o = (const T *)a.out + t * a.os[0] + hd * a.os[1] + lane * E;
         float size = 0.f;
         for (int e = 0; e < E; ++e) size += fabsf(to_f32(o[e]));
-        if (__any_sync(~0u, !(size < INFINITY))) attend_row<D, T, C>(a, s, t, hd, lane);
+        if (__any_sync(~0u, !(size < INFINITY))) attend_mend<D, T, C>(a, t, hd, lane);
     }
 }
 
 // Merges the pieces of a cut tile: block c those of the tile whose first piece CTA c has left.  Piece 0 lies in slot 1 of CTA c,
 // the others in slot 0 of the CTAs behind it.  A warp per row, in the order of the pieces.
 // An infinity or NaN in V at a position that some rows of a tile do not see has met their weight of 0 in the product.  Such
-// rows show it by not being finite; they are done over here, position by position.
+// rows show it by not being finite; they are done over here, position by position: a row of a cut tile by the warp that has
+// joined it, a row of a whole tile, which the kernel in front has stored, by any.
 template <int D, int TY>
 __global__ void __launch_bounds__(256, 3) attend_join_kernel(const __grid_constant__ TcParams p) {
     constexpr int LANES = D / 4, ROWS = 32 / LANES;   // lanes a row, four values each; rows a warp
@@ -1166,15 +1182,15 @@ __global__ void __launch_bounds__(256, 3) attend_join_kernel(const __grid_consta
             o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
             const int row = row0 + tok, head = h * a.group + rr % a.group;
             if (mine) put4<TY>(a.out, row * a.os[0] + head * a.os[1] + ch * 4, o);
-            if (__any_sync(~0u, mine && !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY))) odd = 1;
+            const uint32_t bad = __ballot_sync(~0u, mine && !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY));
+#pragma unroll 1
+            for (int i = 0; i < ROWS; ++i)
+                if (bad >> (i * LANES) & (~0u >> (32 - LANES)))
+                    attend_mend<D, T, C>(a, __shfl_sync(~0u, row, i * LANES), __shfl_sync(~0u, head, i * LANES), lane);
         }
     }
-    // (the rows of other blocks' tiles may still be on their way to `out`: each block looks at its own tile's and at whole tiles')
-    if (__syncthreads_or(odd)) {
-        for (int t = blockIdx.y * gridDim.x + blockIdx.x; t < a.B.rows; t += gridDim.x * gridDim.y) attend_mend<D, T, C>(a, t, warp, lane);
-        if (more > 0)
-            for (int t = row0 + (int)blockIdx.y; t < row0 + ntok; t += gridDim.y) attend_mend<D, T, C>(a, t, warp, lane);
-    }
+    if (__syncthreads_or(odd))
+        for (int t = blockIdx.y * gridDim.x + blockIdx.x; t < a.B.rows; t += gridDim.x * gridDim.y) attend_mend_whole<D, T, C>(p, t, warp, lane);
 }
 
 // ------------------------------------------------------------------------------------------------ launches

@@ -1,0 +1,98 @@
+"""The paged KV cache on a GPU, where its operators could go wrong: what hidden positions hold beside tiles that are cut over
+many blocks, and what the calls report and leave behind."""
+import math
+
+import pytest
+import torch
+
+from tests.pages_util import TY, Pool, attend64, attend_bound
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def G():
+    from allpaka_b200 import gpu
+
+    return gpu
+
+
+@pytest.fixture(scope="module")
+def g(G):
+    ctx = G.Gpu(0)
+    yield ctx
+    ctx.close()
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def ints(a):
+    return torch.tensor(a, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------------------- hidden values beside cut tiles
+
+def hidden_case(G, g, rows, lens, spoils, *, cache, rows_ty, kv, group, dim, window=0, page=16, seed=60):
+    """spoils: (sequence, position, value): V of that position, every head, one dimension.  The output is held against 64
+    bits, with finite values in it beforehand and with NaN, and has the same bits both times."""
+    ty, heads, n = rows_ty or cache, kv * group, len(rows)
+    pool = Pool(1, sum(-(-x // page) for x in lens) + 1, page, kv, dim, cache, n, max(-(-x // page) for x in lens), seed=seed)
+    r = gen(seed)
+    for s, x in enumerate(lens):
+        pool.fill(s, x, r)
+    for s, j, x in spoils:
+        pool.v[0, int(pool.table[s, j // page]), j % page, :, dim // 2 + 3] = x
+    cu = [0]
+    for x in rows:
+        cu.append(cu[-1] + x)
+    q = (torch.randn((cu[-1], heads, dim), generator=r, device="cuda") * 1.5).to(TY[ty])
+    pages, scale, outs = G.KvPages(g, *pool.args()), dim ** -0.5, []
+    for before in (7.0, math.nan):
+        out = torch.full_like(q, before)
+        assert g.attend_pages(pages, 0, q, ints(cu), scale, out, window=window, wait=True), g.last_decline
+        outs.append(out)
+    for s in range(n):
+        part = slice(cu[s], cu[s + 1])
+        k, v = pool.read(s)
+        o, a, most = attend64(q[part], k, v, scale, True, window)
+        got, fine = outs[0][part].double(), torch.isfinite(o)
+        assert torch.equal(torch.isfinite(got), fine), (s, (~torch.isfinite(got) & fine).any(2).nonzero().tolist()[:9])
+        assert float(((got - o).abs() - attend_bound(o, a, most, ty))[fine].max()) <= 0
+    assert torch.equal(outs[0].view(torch.uint8), outs[1].view(torch.uint8))
+    return outs[0]
+
+
+KINDS = [("f16", None), ("bf16", None), ("f16", "f32")]
+
+
+@pytest.mark.parametrize("cache,rows_ty", KINDS)
+@pytest.mark.parametrize("dim,kv,group", [(128, 8, 4), (128, 8, 1), (64, 4, 4), (128, 2, 5), (64, 2, 8), (128, 1, 48)])
+def test_drafts_do_not_see_a_later_drafts_infinity(G, g, cache, rows_ty, dim, kv, group):
+    """Every tile is cut over several blocks; only the last of eight rows sees the infinity."""
+    n, length = 5, 6000
+    out = hidden_case(G, g, [8] * n, [length] * n, [(s, length - 1, math.inf if s % 2 else -math.inf) for s in range(n)], cache=cache, rows_ty=rows_ty,
+                      kv=kv, group=group, dim=dim)
+    assert bool(torch.isfinite(out.view(n, 8, -1)[:, :7]).all())
+
+
+@pytest.mark.parametrize("cache,rows_ty", KINDS)
+@pytest.mark.parametrize("dim,group", [(128, 1), (128, 4), (64, 5), (64, 8), (128, 16)])
+@pytest.mark.parametrize("rows", [1, 5, 8])
+def test_what_lies_before_the_window_does_not_matter(G, g, cache, rows_ty, dim, group, rows):
+    """Cut tiles meet the infinity in their first block, where no row sees it; beside them a clean chunk of many rows."""
+    lens, window = [5003, 4100, 700], 3000
+    spoils = [(s, lens[s] - rows - window, x) for s, x in ((0, -math.inf), (1, math.nan))]
+    for s, j, _ in spoils:   # (the position in front of the first row's window, in the same block of 128)
+        assert j // 128 == (j + 1) // 128
+    out = hidden_case(G, g, [rows, rows, 300], lens, spoils, cache=cache, rows_ty=rows_ty, kv=2, group=group, dim=dim, window=window)
+    assert bool(torch.isfinite(out).all())
+
+
+@pytest.mark.parametrize("cache,rows_ty", KINDS)
+@pytest.mark.parametrize("dim,group", [(128, 4), (64, 7)])
+def test_a_long_chunk_does_not_see_behind_itself(G, g, cache, rows_ty, dim, group):
+    """Tiles of 256 rows, cut; whole ones beside them in the same call."""
+    out = hidden_case(G, g, [200, 1, 90], [9000, 60, 90], [(0, 8990, math.nan), (2, 89, math.inf)], cache=cache, rows_ty=rows_ty, kv=2, group=group, dim=dim)
+    assert bool(torch.isfinite(out[:190]).all()) and bool(torch.isfinite(out[200:290]).all())
