@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <climits>
 
 namespace apk {
 namespace {
@@ -321,19 +322,20 @@ __global__ void __launch_bounds__(256) pages_release_kernel(const __grid_constan
 }
 
 // Inclusive sum over the 1024 threads of a block.
-__device__ __forceinline__ int block_scan(int x, int *sh /*32*/) {
+template <typename T>
+__device__ __forceinline__ T block_scan(T x, T *sh /*32*/) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(~0u, x, o);
+        const T y = __shfl_up_sync(~0u, x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();
     if (lane == 31) sh[warp] = x;
     __syncthreads();
     if (warp == 0) {
-        int w = sh[lane];
+        T w = sh[lane];
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(~0u, w, o);
+            const T y = __shfl_up_sync(~0u, w, o);
             if (lane >= o) w += y;
         }
         sh[lane] = w;
@@ -347,6 +349,7 @@ __device__ __forceinline__ int block_scan(int x, int *sh /*32*/) {
 // keeps the original.  All or nothing: with too few pages nothing changes and work[PW_SHORT] says how many are missing.
 __global__ void __launch_bounds__(PAGES_MAX_LIST) pages_reserve_kernel(const __grid_constant__ PagesDev P, const __grid_constant__ SlotList l) {
     __shared__ int sh[32], last_of[PAGES_MAX_LIST], first_of[PAGES_MAX_LIST], n_copies, too_long;
+    __shared__ long long needs[32];
     const int i = threadIdx.x;
     int *const list = P.work + PW_LIST;
     int *const fresh = list + 4 * P.n_seqs;
@@ -372,9 +375,9 @@ __global__ void __launch_bounds__(PAGES_MAX_LIST) pages_reserve_kernel(const __g
         copy = P.refs[last] - before > 1;
     }
     const int need = i < l.n ? want - have + copy : 0;
-    const int end = block_scan(need, sh);
-    const int total = sh[31];
-    first_of[i] = end - need;
+    const long long end = block_scan((long long)need, needs);   // (64 bits: 1024 sequences of up to 2^27 pages)
+    const long long total = needs[31];
+    first_of[i] = (int)(end - need);   // (used only where all of them are there)
     __syncthreads();
     if (too_long) {
         if (i == 0) { P.work[PW_SHORT] = -1; P.work[PW_COPIES] = 0; }
@@ -390,7 +393,7 @@ __global__ void __launch_bounds__(PAGES_MAX_LIST) pages_reserve_kernel(const __g
         __syncthreads();
     }
     if (got < total) {
-        if (i == 0) { P.work[PW_SHORT] = total - got; P.work[PW_COPIES] = 0; }
+        if (i == 0) { P.work[PW_SHORT] = (int)min(total - got, (long long)INT_MAX); P.work[PW_COPIES] = 0; }
         return;
     }
     __syncthreads();

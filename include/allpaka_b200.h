@@ -442,8 +442,8 @@ typedef struct {
  * free ones, lowest number first, in the order of the list.  A sequence that would write into a last
  * page which others hold too first gets a copy of that page's positions (all layers); of several such
  * sequences in one list the last keeps the original if nobody else holds it.  All or nothing: work[0]
- * becomes 0, or the number of missing pages, or -1 when a row of the table is too short, and then
- * nothing has changed.  wait != 0 synchronises the stream and declines with APK_DECLINE_INVALID_STATE
+ * becomes 0, or the number of missing pages (INT32_MAX for more), or -1 when a row of the table is too
+ * short, and then nothing has changed.  wait != 0 synchronises the stream and declines with APK_DECLINE_INVALID_STATE
  * in the last two cases.  seqs and n_new are HOST arrays; a sequence may be named once. */
 int apk_pages_reserve(apk_ctx *ctx, const apk_pages *pages, uint32_t n, const int32_t *seqs, const int32_t *n_new, void *stream,
                       int wait);

@@ -96,3 +96,19 @@ def test_a_long_chunk_does_not_see_behind_itself(G, g, cache, rows_ty, dim, grou
     """Tiles of 256 rows, cut; whole ones beside them in the same call."""
     out = hidden_case(G, g, [200, 1, 90], [9000, 60, 90], [(0, 8990, math.nan), (2, 89, math.inf)], cache=cache, rows_ty=rows_ty, kv=2, group=group, dim=dim)
     assert bool(torch.isfinite(out[:190]).all()) and bool(torch.isfinite(out[200:290]).all())
+
+
+# ------------------------------------------------------------------------------------------- the pages' upkeep
+
+@pytest.mark.parametrize("n", [15, 18])
+def test_reserve_of_more_pages_than_32_bits_count(G, g, n):
+    """Sequences of 2^30 - 8 positions each: 15 of them ask for fewer than 2^31 pages, 18 for more."""
+    pages, page, width = 6, 8, 2 ** 27 - 1
+    k, v = (torch.zeros((1, pages, page, 1, 8), dtype=torch.float16, device="cuda") for _ in range(2))
+    table = torch.empty((n, width), dtype=torch.int32, device="cuda")
+    lens, refs = ints([0] * n), ints([0, 1, 0, 0, 0, 0])
+    pool = G.KvPages(g, k, v, table, lens, refs)
+    assert not g.pages_reserve(pool, range(n), [width * page] * n) and g.last_decline[0] == 6
+    assert int(pool.short_by) == min(n * width - 5, 2 ** 31 - 1)
+    assert not bool(lens.any()) and refs.tolist() == [0, 1, 0, 0, 0, 0]
+    assert g.pages_reserve(pool, range(n), [9] + [0] * (n - 1)) and table[0, :2].tolist() == [0, 2]
