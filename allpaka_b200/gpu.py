@@ -498,6 +498,8 @@ class KvPages:
         S, W = table.shape
         if W > 1 and table.stride(1) != 1:
             raise ValueError("the rows of the page table are not contiguous")
+        if S > 1 and table.stride(0) < W:
+            raise ValueError("the rows of the page table overlap")
         _tensor(lens, "lens", (S,), "torch.int32", dev)
         _tensor(refs, "refs", (NP,), "torch.int32", dev)
         self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs

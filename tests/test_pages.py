@@ -101,6 +101,16 @@ def test_a_pool_of_the_wrong_tensors(gpu, ctx):
             pool(gpu, ctx, **bad)
 
 
+def test_a_table_whose_rows_overlap(gpu, ctx):
+    """One row for all sequences (an expanded tensor): its storage ends long before the last row of a table would."""
+    for stride in ((0, 1), (4, 1)):
+        with pytest.raises(ValueError):
+            pool(gpu, ctx, table=Tensor(3, 5, dtype="int32", stride=stride))
+    one = pool(gpu, ctx, table=Tensor(1, 5, dtype="int32", stride=(0, 1)), lens=Tensor(1, dtype="int32"))
+    assert one._c.table_stride == 5
+    assert pool(gpu, ctx, table=Tensor(3, 5, dtype="int32", stride=(9, 1)))._c.table_stride == 9
+
+
 @pytest.mark.parametrize("kw,code", [(dict(page=24), 3), (dict(page=4), 3), (dict(page=512), 3), (dict(dim=20), 3), (dict(dim=264), 3),
                                      (dict(k=Tensor(2, 10, 16, 2, 128, ptr=(1 << 20) + 8)), 3),
                                      (dict(k=Tensor(2, 10, 16, 2, 128, stride=(41000, 4100, 256, 128, 1))), 3), (dict(width=1 << 27), 3)])
