@@ -347,7 +347,8 @@ __device__ __forceinline__ T block_scan(T x, T *sh /*32*/) {
 // Room for b more positions in each listed sequence: thread i looks after entry i.  A sequence that is about to write
 // into a last page which others hold too gets a copy of it; in the order of the list, so the last of several holders
 // keeps the original.  All or nothing: with too few pages nothing changes and work[PW_SHORT] says how many are missing.
-__global__ void __launch_bounds__(PAGES_MAX_LIST) pages_reserve_kernel(const __grid_constant__ PagesDev P, const __grid_constant__ SlotList l) {
+// heed: with an expired wait of an earlier call to report, nothing changes either.
+__global__ void __launch_bounds__(PAGES_MAX_LIST) pages_reserve_kernel(const __grid_constant__ PagesDev P, const __grid_constant__ SlotList l, int heed) {
     __shared__ int sh[32], last_of[PAGES_MAX_LIST], first_of[PAGES_MAX_LIST], n_copies, too_long;
     __shared__ long long needs[32];
     const int i = threadIdx.x;
@@ -355,6 +356,10 @@ __global__ void __launch_bounds__(PAGES_MAX_LIST) pages_reserve_kernel(const __g
     int *const fresh = list + 4 * P.n_seqs;
     pages_let_next();
     pages_wait_front();
+    if (heed && P.work[PW_ERR]) {
+        if (i == 0) { P.work[PW_SHORT] = PW_UNTRIED; P.work[PW_COPIES] = 0; }
+        return;
+    }
     if (i == 0) n_copies = too_long = 0;
     int slot = 0, old = 0, have = 0, want = 0, last = -1;
     if (i < l.n) {
@@ -556,9 +561,9 @@ cudaError_t launch_pages_release(const PagesDev &P, const SlotList &l, cudaStrea
     return launch_front(pages_release_kernel, dim3(l.n), 256, 0, st, P, l);
 }
 
-cudaError_t launch_pages_reserve(const PagesDev &P, const SlotList &l, int n_sm, cudaStream_t st, int *launches) {
+cudaError_t launch_pages_reserve(const PagesDev &P, const SlotList &l, int heed, int n_sm, cudaStream_t st, int *launches) {
     *launches += 1;
-    cudaError_t e = launch_front(pages_reserve_kernel, dim3(1), PAGES_MAX_LIST, 0, st, P, l);
+    cudaError_t e = launch_front(pages_reserve_kernel, dim3(1), PAGES_MAX_LIST, 0, st, P, l, heed);
     if (e != cudaSuccess || l.n == 0) return e;
     *launches += 1;
     return launch_front(pages_copy_kernel, dim3(copy_blocks(P, l.n, n_sm)), 256, 0, st, P);

@@ -19,10 +19,11 @@ constexpr int PAGES_MAX_LIST = 1024;   // sequences that one reserve, fork or re
 constexpr int PAGES_MAX_BATCH = 4096;  // sequences of one batch of rows
 
 // work[]: what the kernels of one pool hand on to one another
-constexpr int PW_SHORT = 0;    // reserve: pages that were missing (0: done, -1: a row of the table is too short)
+constexpr int PW_SHORT = 0;    // reserve: pages that were missing (0: done, -1: a row of the table is too short, PW_UNTRIED)
 constexpr int PW_ERR = 1;      // a wait inside a kernel ran out (stays until it has been reported)
 constexpr int PW_COPIES = 2;   // entries of the copy list
 constexpr int PW_LIST = 64;    // n_seqs x {source page, destination page, positions, 0}, then the page lists
+constexpr int PW_UNTRIED = -2; // in work[PW_SHORT]: reserve has changed nothing, because an expired wait is to be reported
 
 struct PagesDev {
     uint16_t *k, *v;            // 16-bit elements
@@ -141,7 +142,7 @@ size_t attend_ws_bytes(const AttendParams &p, int n_sm);
 cudaError_t launch_attend(const AttendParams &p, int n_sm, void *ws, long long wait_limit, cudaStream_t st, int *launches);
 cudaError_t launch_pages_fork(const PagesDev &P, const SlotList &l, cudaStream_t st, int *launches);
 cudaError_t launch_pages_release(const PagesDev &P, const SlotList &l, cudaStream_t st, int *launches);
-cudaError_t launch_pages_reserve(const PagesDev &P, const SlotList &l, int n_sm, cudaStream_t st, int *launches);
+cudaError_t launch_pages_reserve(const PagesDev &P, const SlotList &l, int heed, int n_sm, cudaStream_t st, int *launches);
 cudaError_t launch_pages_compact(const PagesDev &P, int *page_map, int n_sm, cudaStream_t st, int *launches);
 
 }  // namespace apk

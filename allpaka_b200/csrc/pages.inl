@@ -112,12 +112,13 @@ int pages_distinct(const char *what, const int32_t *a, uint32_t n) {
     return APK_OK;
 }
 
-// What a waited call reports: the words of work[] after its kernels.
+// What a waited call reports: the words of work[] after its kernels.  A reservation reports an expired wait only where it has
+// changed nothing on that account: its caller repeats what ends in an error.
 int pages_wait(const char *what, const PagesDev &P, cudaStream_t st, bool reserve) {
     int w[2] = {0, 0};
     CUDA_TRY(cudaMemcpyAsync(w, P.work, sizeof w, cudaMemcpyDeviceToHost, st));
     CUDA_TRY(cudaStreamSynchronize(st));
-    if (w[PW_ERR]) {
+    if (reserve ? w[PW_SHORT] == PW_UNTRIED : w[PW_ERR] != 0) {
         CUDA_TRY(cudaMemsetAsync(P.work + PW_ERR, 0, sizeof(int), st));
         CUDA_TRY(cudaStreamSynchronize(st));
         return fail(APK_ERR_TIMEOUT, "%s: device-side wait expired (site %d)", what, w[PW_ERR]);
@@ -223,7 +224,9 @@ int apk_rope_append(apk_ctx *c, const apk_rope_req *r, void *stream, int wait) {
     int launches = 0;
     const cudaError_t e = launch_rope_append(p, c->n_sm, (cudaStream_t)stream, &launches);
     APK_TRY(pages_done(c, e, launches, what));
-    return wait ? pages_wait(what, p.P, (cudaStream_t)stream, false) : APK_OK;
+    // (it has no waits of its own to report, and one in place may not be repeated)
+    if (wait) CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
+    return APK_OK;
 }
 
 }  // extern "C"
@@ -306,7 +309,7 @@ int apk_pages_reserve(apk_ctx *c, const apk_pages *pages, uint32_t n, const int3
     DeviceScope dev;
     CUDA_TRY(dev.enter(c->device));
     int launches = 0;
-    const cudaError_t e = launch_pages_reserve(P, l, c->n_sm, (cudaStream_t)stream, &launches);
+    const cudaError_t e = launch_pages_reserve(P, l, wait != 0, c->n_sm, (cudaStream_t)stream, &launches);
     APK_TRY(pages_done(c, e, launches, what));
     return wait ? pages_wait(what, P, (cudaStream_t)stream, true) : APK_OK;
 }

@@ -506,7 +506,7 @@ class KvPages:
         self.n_layers, self.n_pages, self.page, self.n_kv_heads, self.head_dim = L, NP, page, H, D
         self.device, self.n_seqs, self.width = dev, S, W
         self.work = refs.new_zeros(64 + 4 * S + 3 * NP)
-        #: what the last :meth:`Gpu.pages_reserve` reported, on the device: 0, the pages that were missing, or -1
+        #: what the last :meth:`Gpu.pages_reserve` reported, on the device: 0, the pages that were missing, -1 or -2
         self.short_by = self.work[0]
         self._c = _Pages(k.data_ptr(), v.data_ptr(), _TENSOR_TY[_DTYPE[k.dtype]], L, NP, page, H, D,
                          (C.c_uint64 * 4)(*k.stride()[:4]), (C.c_uint64 * 4)(*v.stride()[:4]), table.data_ptr(),
@@ -866,7 +866,8 @@ class Gpu:
 
     def pages_reserve(self, pages: KvPages, seqs, n_new, stream: Optional[int] = None, wait: bool = True) -> bool:
         """``apk_pages_reserve``: room for ``n_new[i]`` more positions in sequence ``seqs[i]`` (host lists).  False when pages are
-        missing or a row of the table is too short, and then nothing has changed; with ``wait`` off ``pages.short_by`` says so."""
+        missing or a row of the table is too short, and then nothing has changed; with ``wait`` off ``pages.short_by`` says so.  With
+        ``wait`` on, an expired wait of an earlier :meth:`attend_pages` is raised here, and then nothing has changed either."""
         a, b = self._lists(pages, seqs, n_new)
         return self._check(self._l.apk_pages_reserve(self._h, pages._p, len(a) // 4, a, b,
                                                      _stream(stream, pages.work), 1 if wait else 0))

@@ -443,8 +443,10 @@ typedef struct {
  * page which others hold too first gets a copy of that page's positions (all layers); of several such
  * sequences in one list the last keeps the original if nobody else holds it.  All or nothing: work[0]
  * becomes 0, or the number of missing pages (INT32_MAX for more), or -1 when a row of the table is too
- * short, and then nothing has changed.  wait != 0 synchronises the stream and declines with APK_DECLINE_INVALID_STATE
- * in the last two cases.  seqs and n_new are HOST arrays; a sequence may be named once. */
+ * short, and then nothing has changed.  wait != 0 synchronises the stream and declines with
+ * APK_DECLINE_INVALID_STATE in the last two cases; where an earlier apk_attend_pages on the pool that was
+ * not waited for let a device-side wait expire, it reports that instead (APK_ERR_TIMEOUT), work[0] is -2,
+ * and nothing has changed.  seqs and n_new are HOST arrays; a sequence may be named once. */
 int apk_pages_reserve(apk_ctx *ctx, const apk_pages *pages, uint32_t n, const int32_t *seqs, const int32_t *n_new, void *stream,
                       int wait);
 /* Sequence dst[i] becomes a second holder of src[i]'s positions, in place of what it held.  No page is
@@ -483,7 +485,7 @@ typedef struct {
  * rounded once.  Rows cu[i] .. cu[i+1]-1 are the LAST positions of sequence seqs[i] (its length counts
  * them already: apk_pages_reserve): row cu[i] + j stands at position lens - rows + j.  It turns by
  * that position, or by positions[row] if given.  Rows that belong to no sequence are left alone.
- * A sequence may be named once. */
+ * A sequence may be named once.  wait != 0: synchronises the stream. */
 typedef struct {
     const apk_pages *pages;
     uint32_t layer;
@@ -530,7 +532,8 @@ typedef struct {
 /* The scratch a request needs (its pointers are not read); 0 for one that would be refused. */
 size_t apk_attend_pages_ws(apk_ctx *ctx, const apk_attend_req *req);
 /* wait != 0: synchronises the stream and reports an expired device-side wait (APK_ERR_TIMEOUT; one of
- * an earlier call that was not waited for is reported by the next one on the pool that is). */
+ * an earlier call that was not waited for is reported by the next one on the pool that is, or by a waited
+ * apk_pages_reserve). */
 int apk_attend_pages(apk_ctx *ctx, const apk_attend_req *req, void *stream, int wait);
 
 /* Human-readable reason for the last non-zero status on this thread

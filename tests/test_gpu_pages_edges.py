@@ -112,3 +112,28 @@ def test_reserve_of_more_pages_than_32_bits_count(G, g, n):
     assert int(pool.short_by) == min(n * width - 5, 2 ** 31 - 1)
     assert not bool(lens.any()) and refs.tolist() == [0, 1, 0, 0, 0, 0]
     assert g.pages_reserve(pool, range(n), [9] + [0] * (n - 1)) and table[0, :2].tolist() == [0, 2]
+
+
+def test_an_earlier_calls_expired_wait_and_a_reservation(G, g):
+    """work[1] is where attention leaves an expired wait (planted here).  A waited reservation that reports it has changed
+    nothing, so it can be repeated; one that is not waited for does its work and leaves the report to the next waited call."""
+    pool = Pool(1, 20, 16, 2, 64, "f16", 2, 8, seed=70)
+    r = gen(70)
+    pool.fill(0, 30, r)
+    pages = G.KvPages(g, *pool.args())
+    refs, table = pool.refs.clone(), pool.table.clone()
+    pages.work[1] = 7
+    with pytest.raises(G.GpuError) as e:
+        g.pages_reserve(pages, [0, 1], [10, 5])
+    assert e.value.code == -3 and int(pages.short_by) == -2
+    assert pool.lens.tolist() == [30, 0] and torch.equal(pool.refs, refs) and torch.equal(pool.table, table)
+    assert g.pages_reserve(pages, [0, 1], [10, 5]) and pool.lens.tolist() == [40, 5] and int(pages.short_by) == 0
+    pages.work[1] = 7
+    assert g.pages_reserve(pages, [0, 1], [1, 1], wait=False) and int(pages.short_by) == 0 and pool.lens.tolist() == [41, 6]
+    x = [torch.randn((2, h, 64), generator=r, device="cuda").half() for h in (4, 2, 2)]
+    turned = torch.empty_like(x[0])
+    assert g.rope_append(pages, 0, *x, ints([0, 1, 2]), None, out=turned, wait=True) and torch.equal(turned, x[0])
+    with pytest.raises(G.GpuError) as e:
+        g.attend_pages(pages, 0, turned, ints([0, 1, 2]), 0.1, torch.empty_like(turned), wait=True)
+    assert e.value.code == -3
+    assert g.attend_pages(pages, 0, turned, ints([0, 1, 2]), 0.1, torch.empty_like(turned), wait=True)
