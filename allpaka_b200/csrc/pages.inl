@@ -192,7 +192,8 @@ int apk_rope_append(apk_ctx *c, const apk_rope_req *r, void *stream, int wait) {
     RopeParams p{};
     APK_TRY(pages_view(what, r->pages, &p.P));
     APK_TRY(pages_batch(what, r->cu, r->seqs, r->n, r->n_rows, &p.B));
-    if (!r->k || !r->v || (r->q && !r->out)) return fail(APK_ERR_INVALID_ARG, "%s: null rows", what);
+    const bool none = r->n == 0 || r->n_rows == 0;   // (rows that are not there may have no address)
+    if (!none && (!r->k || !r->v || (r->q && !r->out))) return fail(APK_ERR_INVALID_ARG, "%s: null rows", what);
     if (r->layer >= r->pages->n_layers) return fail(APK_ERR_INVALID_ARG, "%s: layer %u of %u", what, r->layer, r->pages->n_layers);
     APK_TRY(check_rows(what, "k", r->k, r->ty, r->k_stride));
     APK_TRY(check_rows(what, "v", r->v, r->ty, r->v_stride));
@@ -200,7 +201,7 @@ int apk_rope_append(apk_ctx *c, const apk_rope_req *r, void *stream, int wait) {
         if (r->n_heads == 0 || r->n_heads > 65535) return fail(APK_DECLINE_UNSUPPORTED_SHAPE, "%s: %u heads", what, r->n_heads);
         APK_TRY(check_rows(what, "q", r->q, r->ty, r->q_stride));
         APK_TRY(check_rows(what, "out", r->out, r->out_ty, r->out_stride));
-        if (r->out == r->q && (r->out_ty != r->ty || r->out_stride[0] != r->q_stride[0] || r->out_stride[1] != r->q_stride[1]))
+        if (!none && r->out == r->q && (r->out_ty != r->ty || r->out_stride[0] != r->q_stride[0] || r->out_stride[1] != r->q_stride[1]))
             return fail(APK_ERR_INVALID_ARG, "%s: out in place of q has its type and strides", what);
     }
     if ((r->q_norm || r->k_norm) && !(r->eps >= 0.f)) return fail(APK_ERR_INVALID_ARG, "%s: eps %g", what, r->eps);
@@ -218,7 +219,7 @@ int apk_rope_append(apk_ctx *c, const apk_rope_req *r, void *stream, int wait) {
     p.q_norm = r->q_norm;
     p.k_norm = r->k_norm;
     p.eps = r->eps;
-    if (r->n == 0 || r->n_rows == 0) return APK_OK;
+    if (none) return APK_OK;
     DeviceScope dev;
     CUDA_TRY(dev.enter(c->device));
     int launches = 0;
@@ -238,7 +239,8 @@ int attend_view(const apk_attend_req *r, AttendParams *q) {
     AttendParams &p = *q;
     APK_TRY(pages_view(what, r->pages, &p.P));
     APK_TRY(pages_batch(what, r->cu, r->seqs, r->n, r->n_rows, &p.B));
-    if (!r->q || !r->out) return fail(APK_ERR_INVALID_ARG, "%s: null rows", what);
+    const bool none = r->n == 0 || r->n_rows == 0;   // (rows that are not there may have no address)
+    if (!none && (!r->q || !r->out)) return fail(APK_ERR_INVALID_ARG, "%s: null rows", what);
     if (r->layer >= r->pages->n_layers) return fail(APK_ERR_INVALID_ARG, "%s: layer %u of %u", what, r->layer, r->pages->n_layers);
     APK_TRY(check_rows(what, "q", r->q, r->ty, r->q_stride));
     APK_TRY(check_rows(what, "out", r->out, r->ty, r->out_stride));
@@ -246,7 +248,7 @@ int attend_view(const apk_attend_req *r, AttendParams *q) {
         return fail(APK_DECLINE_UNSUPPORTED_TYPE, "%s: rows of type %u over pages of type %u (the pages' type, or f32 over f16)", what, r->ty, r->pages->ty);
     if (r->pages->head_dim != 64 && r->pages->head_dim != 128)
         return fail(APK_DECLINE_UNSUPPORTED_SHAPE, "%s: heads of %u dimensions (64 and 128 are supported)", what, r->pages->head_dim);
-    if (r->out == r->q) return fail(APK_ERR_INVALID_ARG, "%s: out in place of q", what);
+    if (!none && r->out == r->q) return fail(APK_ERR_INVALID_ARG, "%s: out in place of q", what);
     const uint32_t kv = r->pages->n_kv_heads;
     if (r->n_heads == 0 || r->n_heads % kv || r->n_heads / kv > 64)
         return fail(APK_DECLINE_UNSUPPORTED_SHAPE, "%s: %u heads over %u kv heads (whole groups of at most 64)", what, r->n_heads, kv);

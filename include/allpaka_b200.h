@@ -418,7 +418,8 @@ void apk_stats(apk_ctx *ctx, apk_stats_t *out);
  * Nothing that the device arrays hold can lead outside the buffers: a page number outside the pool is
  * a page that is not there (its positions are not visible, stores to it are dropped), a length is cut
  * to the row of the table, a sequence number outside the table has no positions, row offsets are cut to
- * n_rows (they rise; what rows get that several sequences claim is not defined). */
+ * n_rows (they rise; what rows get that several sequences claim is not defined).
+ * A batch of no rows or no sequences is nothing to do; its rows may be NULL. */
 #define APK_PAGES_MAX_LIST 1024u  /* sequences one _reserve, _fork or _release names */
 #define APK_PAGES_MAX_BATCH 4096u /* sequences of one _rope_append or _attend */
 /* int32 values of apk_pages.work, the pool's scratch: zeroed by the caller once, then left alone */

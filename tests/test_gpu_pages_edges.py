@@ -137,3 +137,13 @@ def test_an_earlier_calls_expired_wait_and_a_reservation(G, g):
         g.attend_pages(pages, 0, turned, ints([0, 1, 2]), 0.1, torch.empty_like(turned), wait=True)
     assert e.value.code == -3
     assert g.attend_pages(pages, 0, turned, ints([0, 1, 2]), 0.1, torch.empty_like(turned), wait=True)
+
+
+def test_a_step_without_rows(G, g):
+    pool = Pool(1, 4, 16, 2, 64, "f16", 2, 2, seed=71)
+    pages = G.KvPages(g, *pool.args())
+    q, k = (torch.empty((0, h, 64), dtype=torch.float16, device="cuda") for h in (4, 2))
+    for cu, seqs in ((ints([0]), None), (ints([0, 0, 0]), ints([1, 0]))):
+        assert g.rope_append(pages, 0, q, k, k, cu, G.Rope(64), seqs=seqs, wait=True)
+        assert g.attend_pages(pages, 0, q, cu, 0.1, torch.empty_like(q), seqs=seqs, wait=True)
+    assert g.pages_reserve(pages, [0, 1], [0, 0]) and not bool(pool.refs.any())

@@ -169,6 +169,22 @@ def test_attention_requests_that_are_refused(gpu, ctx):
     assert attend(ctx, p, q=Tensor(0, 8, 128)) and attend(ctx, p, cu=Tensor(1, dtype="int32"))   # no rows, no sequences
 
 
+def test_batches_without_rows_are_nothing_to_do(gpu, ctx):
+    """A tensor without elements has no address (0)."""
+    p = pool(gpu, ctx)
+    none = {h: Tensor(0, h, 128, ptr=0) for h in (8, 2)}
+    for n in (1, 3):
+        cu = Tensor(n, dtype="int32")
+        assert attend(ctx, p, q=none[8], out=none[8], cu=cu)
+        for q in (none[8], None):
+            for out in (None, none[8]):
+                assert ctx.rope_append(p, 0, q, none[2], none[2], cu, gpu.Rope(64), out=out, stream=0)
+    with pytest.raises(ValueError):
+        attend(ctx, p, q=none[8], out=Tensor(1, 8, 128))
+    with pytest.raises(gpu.GpuError):   # rows without an address
+        attend(ctx, p, q=Tensor(4, 8, 128, ptr=0))
+
+
 def rope_call(ctx, p, rope, q=None, k=None, v=None, out=None, **kw):
     q, k, v = q or Tensor(4, 8, 128), k or Tensor(4, 2, 128), v or Tensor(4, 2, 128)
     return ctx.rope_append(p, 0, q, k, v, Tensor(3, dtype="int32"), rope, out=out or Tensor(4, 8, 128, ptr=2 << 20), stream=0, **kw)
