@@ -431,6 +431,16 @@ def _current_stream(device: int) -> int:
     return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
+def _settle(t) -> None:
+    """Waits until the device has filled ``t``, so that any stream may use it (in a capture the zeros are the graph's)."""
+    if getattr(t, "is_cuda", False):
+        import torch
+
+        with torch.cuda.device(t.device):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
+
+
 def _list32(a) -> bytes:
     """A host list of 32-bit integers, as the C side reads it."""
     if isinstance(a, (list, tuple, range)):
@@ -482,8 +492,9 @@ class KvPages:
     ``lens``        [n_seqs] int32: positions of each sequence
     ``refs``        [n_pages] int32: sequences that hold the page; 0 = free
 
-    An empty pool has zeros in ``lens`` and ``refs``.  The pool keeps the tensors alive; :meth:`Gpu.pages_reserve` and its
-    companions change them in place, in the order of the stream they are given."""
+    An empty pool has zeros in ``lens`` and ``refs``.  The pool keeps the tensors alive, and is itself kept until its last
+    call has run; :meth:`Gpu.pages_reserve` and its companions change them in place, in the order of the stream they are
+    given, which may be any: the pool's own scratch is ready when the constructor returns."""
 
     def __init__(self, gpu: "Gpu", k, v, table, lens, refs):
         dev = gpu.device
@@ -506,6 +517,7 @@ class KvPages:
         self.n_layers, self.n_pages, self.page, self.n_kv_heads, self.head_dim = L, NP, page, H, D
         self.device, self.n_seqs, self.width = dev, S, W
         self.work = refs.new_zeros(64 + 4 * S + 3 * NP)
+        _settle(self.work)
         #: what the last :meth:`Gpu.pages_reserve` reported, on the device: 0, the pages that were missing, -1 or -2
         self.short_by = self.work[0]
         self._c = _Pages(k.data_ptr(), v.data_ptr(), _TENSOR_TY[_DTYPE[k.dtype]], L, NP, page, H, D,

@@ -147,3 +147,25 @@ def test_a_step_without_rows(G, g):
         assert g.rope_append(pages, 0, q, k, k, cu, G.Rope(64), seqs=seqs, wait=True)
         assert g.attend_pages(pages, 0, q, cu, 0.1, torch.empty_like(q), seqs=seqs, wait=True)
     assert g.pages_reserve(pages, [0, 1], [0, 0]) and not bool(pool.refs.any())
+
+
+def test_a_pool_made_on_a_busy_stream_is_used_on_another(G, g):
+    """Forks and their copies on a side stream, right after the pool was made on a stream with work in front of it."""
+    pool = Pool(2, 40, 16, 2, 64, "f16", 9, 3, seed=72)
+    r = gen(72)
+    held = pool.fill(0, 25, r)
+    pool.k[1], pool.v[1] = pool.k[0], pool.v[0]
+    big = torch.randn((8192, 8192), device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(8):
+        big = big @ big * 1e-4
+    pages, st = G.KvPages(g, *pool.args()), torch.cuda.Stream()
+    kids = list(range(1, 9))
+    assert g.pages_fork(pages, [0] * 8, kids, stream=st.cuda_stream)
+    assert g.pages_reserve(pages, kids, [1] * 8, stream=st.cuda_stream, wait=False)
+    torch.cuda.synchronize()
+    assert int(pages.short_by) == 0 and pool.lens.tolist() == [25] + [26] * 8
+    for s in kids:
+        for layer in (0, 1):
+            k, v = pool.read(s, layer)
+            assert torch.equal(k[:25], held[0]) and torch.equal(v[:25], held[1])
