@@ -454,11 +454,11 @@ def _list32(a) -> bytes:
     return a.reshape(-1).astype(np.int32).tobytes()
 
 
-@dataclass
+@dataclass(frozen=True)
 class Rope:
     """Rotary positions (``apk_rope``): ``dim`` of a head's dimensions turn, as ``"half"`` pairs (i, i + dim/2) or as
     neighbouring ``"pairs"`` (2i, 2i + 1); ``scaling`` "none", "linear" or "yarn" stretches them over a longer context.
-    The frequencies are in the C header."""
+    The frequencies are in the C header.  Fixed once made: ``dataclasses.replace`` makes a changed one."""
     dim: int
     layout: str = "half"
     base: float = 10000.0
@@ -473,14 +473,15 @@ class Rope:
     def __post_init__(self):
         if self.layout not in ("half", "pairs") or self.scaling not in ("none", "linear", "yarn"):
             raise ValueError(f"layout {self.layout!r}, scaling {self.scaling!r}")
-        self._ff = None
+        ff = None
         if self.freq_factors is not None:
-            self._ff = _f32(self.freq_factors).reshape(-1)
-            if self._ff.size != self.dim // 2:
-                raise ValueError(f"{self._ff.size} frequency factors, expected {self.dim // 2}")
-        self._c = _Rope(self.dim, ("half", "pairs").index(self.layout), ("none", "linear", "yarn").index(self.scaling), self.base,
-                        self.factor, self.attn_factor, self.beta_fast, self.beta_slow, self.orig_ctx, _ptr(self._ff))
-        self._p = C.addressof(self._c)
+            ff = _f32(self.freq_factors).reshape(-1).copy()
+            if ff.size != self.dim // 2:
+                raise ValueError(f"{ff.size} frequency factors, expected {self.dim // 2}")
+        c = _Rope(self.dim, ("half", "pairs").index(self.layout), ("none", "linear", "yarn").index(self.scaling), self.base,
+                  self.factor, self.attn_factor, self.beta_fast, self.beta_slow, self.orig_ctx, _ptr(ff))
+        for name, value in (("_ff", ff), ("_c", c), ("_p", C.addressof(c))):
+            object.__setattr__(self, name, value)
 
 
 class KvPages:
@@ -494,7 +495,16 @@ class KvPages:
 
     An empty pool has zeros in ``lens`` and ``refs``.  The pool keeps the tensors alive, and is itself kept until its last
     call has run; :meth:`Gpu.pages_reserve` and its companions change them in place, in the order of the stream they are
-    given, which may be any: the pool's own scratch is ready when the constructor returns."""
+    given, which may be any: the pool's own scratch is ready when the constructor returns.  What it was made of stays."""
+
+    #: what the C side has been told: fixed once made
+    _FIXED = frozenset(("k", "v", "table", "lens", "refs", "work", "short_by", "n_layers", "n_pages", "page", "n_kv_heads", "head_dim",
+                        "n_seqs", "width"))
+
+    def __setattr__(self, name, value):
+        if name in self._FIXED and name in self.__dict__:
+            raise AttributeError(f"{name} of a pool is fixed: make another KvPages")
+        super().__setattr__(name, value)
 
     def __init__(self, gpu: "Gpu", k, v, table, lens, refs):
         dev = gpu.device

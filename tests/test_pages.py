@@ -211,6 +211,22 @@ def test_rotations_that_are_refused(gpu, ctx):
         rope_call(ctx, p, gpu.Rope(64), out=Tensor(4, 8, 128, dtype="float32"))   # in place, but of another type
 
 
+def test_what_has_been_told_to_the_c_side_cannot_be_changed(gpu, ctx):
+    """Neither a rotation nor a pool takes a later assignment that its calls would not follow."""
+    import dataclasses
+
+    rope = gpu.Rope(64, scaling="linear", factor=2.0, freq_factors=[1.0] * 32)
+    for name in ("dim", "layout", "base", "scaling", "factor", "orig_ctx", "beta_fast", "beta_slow", "attn_factor", "freq_factors"):
+        with pytest.raises(AttributeError):
+            setattr(rope, name, getattr(rope, name))
+    other = dataclasses.replace(rope, factor=4.0)
+    assert (rope._c.factor, other._c.factor, other._c.rot_dim) == (2.0, 4.0, 64) and other._p == C.addressof(other._c) != rope._p
+    p = pool(gpu, ctx)
+    for name in ("k", "v", "table", "lens", "refs", "work", "short_by", "n_layers", "n_pages", "page", "n_kv_heads", "head_dim", "n_seqs", "width"):
+        with pytest.raises(AttributeError):
+            setattr(p, name, getattr(p, name))
+
+
 def test_null_requests_are_refused(gpu):
     lib, block = gpu.load_library(), C.create_string_buffer(1 << 16)
     h = C.addressof(block)
