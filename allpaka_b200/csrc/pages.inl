@@ -252,7 +252,8 @@ int attend_view(const apk_attend_req *r, AttendParams *q) {
     const uint32_t kv = r->pages->n_kv_heads;
     if (r->n_heads == 0 || r->n_heads % kv || r->n_heads / kv > 64)
         return fail(APK_DECLINE_UNSUPPORTED_SHAPE, "%s: %u heads over %u kv heads (whole groups of at most 64)", what, r->n_heads, kv);
-    if (!std::isfinite(r->scale)) return fail(APK_ERR_INVALID_ARG, "%s: scale %g", what, r->scale);
+    p.scale_log2 = r->scale * 1.44269504088896340736f;
+    if (!std::isfinite(p.scale_log2)) return fail(APK_ERR_INVALID_ARG, "%s: scale %g", what, r->scale);
     if (r->window >= (1u << 30)) return fail(APK_DECLINE_UNSUPPORTED_SHAPE, "%s: a window of %u", what, r->window);
     p.layer = (int)r->layer;
     p.q = r->q; p.out = r->out;
@@ -260,7 +261,6 @@ int attend_view(const apk_attend_req *r, AttendParams *q) {
     for (int i = 0; i < 2; ++i) { p.qs[i] = (long long)r->q_stride[i]; p.os[i] = (long long)r->out_stride[i]; }
     p.heads = (int)r->n_heads;
     p.group = (int)(r->n_heads / kv);
-    p.scale_log2 = r->scale * 1.44269504088896340736f;
     p.causal = r->causal != 0;
     p.window = (int)r->window;
     // the kernels count (kv head, tile of rows, 128 positions) in 32 bits

@@ -227,6 +227,16 @@ def test_what_has_been_told_to_the_c_side_cannot_be_changed(gpu, ctx):
             setattr(p, name, getattr(p, name))
 
 
+def test_a_scale_beyond_32_bits_is_refused(gpu, ctx):
+    """The kernels work in powers of two: it is the scale times log2(e) that has to be finite."""
+    p = pool(gpu, ctx)
+    for scale in (3e38, -3e38):
+        with pytest.raises(gpu.GpuError) as e:
+            attend(ctx, p, scale=scale)
+        assert e.value.code == -1 and "scale" in str(e.value)
+    assert attend(ctx, p, q=Tensor(0, 8, 128, ptr=0), scale=2e38)
+
+
 def test_null_requests_are_refused(gpu):
     lib, block = gpu.load_library(), C.create_string_buffer(1 << 16)
     h = C.addressof(block)
