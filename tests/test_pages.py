@@ -237,6 +237,24 @@ def test_a_scale_beyond_32_bits_is_refused(gpu, ctx):
     assert attend(ctx, p, q=Tensor(0, 8, 128, ptr=0), scale=2e38)
 
 
+def test_long_lists_that_are_refused(gpu, ctx):
+    """A thousand sequences in any order: one named twice, or forked and written, wherever it stands."""
+    import random
+
+    p, rnd = pool(gpu, ctx, table=Tensor(3000, 5, dtype="int32"), lens=Tensor(3000, dtype="int32")), random.Random(3)
+    some = rnd.sample(range(3000), 2048)
+    src, dst = some[:1024], some[1024:]
+    for i, j in ((0, 1023), (1023, 0), (511, 512), (7, 900)):
+        twice, both = list(dst), list(src)
+        twice[i] = dst[j]
+        both[i] = dst[j]
+        for call, word in ((lambda: ctx.pages_fork(p, src, twice, stream=0), "twice"), (lambda: ctx.pages_reserve(p, twice, [1] * 1024, stream=0), "twice"),
+                           (lambda: ctx.pages_release(p, twice, [0] * 1024, stream=0), "twice"), (lambda: ctx.pages_fork(p, both, dst, stream=0), "both")):
+            with pytest.raises(gpu.GpuError) as e:
+                call()
+            assert e.value.code == -1 and word in str(e.value) and str(dst[j]) in str(e.value)
+
+
 def test_null_requests_are_refused(gpu):
     lib, block = gpu.load_library(), C.create_string_buffer(1 << 16)
     h = C.addressof(block)
