@@ -169,3 +169,33 @@ def test_a_pool_made_on_a_busy_stream_is_used_on_another(G, g):
         for layer in (0, 1):
             k, v = pool.read(s, layer)
             assert torch.equal(k[:25], held[0]) and torch.equal(v[:25], held[1])
+
+
+def test_an_expired_wait_in_attention_is_reported_and_the_pool_lives_on(G):
+    """Sixteen million rows of one sequence, nearly all before its position 0: the warp that looks for a block's share of the work
+    walks 65536 tiles before it hands out the first one, milliseconds, and the others' waits for it run out under a budget
+    of a cycle.  The call reports it, a second one with the ordinary budget is right."""
+    g = G.Gpu(0)
+    rows, length = 1 << 24, 40
+    pool = Pool(1, 4, 16, 1, 64, "f16", 1, 3, seed=73)
+    r = gen(73)
+    k, v = pool.fill(0, length, r)
+    pages = G.KvPages(g, *pool.args())
+    row = torch.randn((1, 1, 64), generator=r, device="cuda").half()
+    q, out = row.expand(rows, 1, 64), torch.full((rows, 1, 64), 7.0, dtype=torch.float16, device="cuda")
+    call = lambda **kw: g.attend_pages(pages, 0, q, ints([0, rows]), 0.1, out, **kw)  # noqa: E731
+    g.debug_set_wait_limit(1)
+    with pytest.raises(G.GpuError) as e:
+        call(wait=True)
+    assert e.value.code == -3 and "site 10" in str(e.value)
+    assert call(wait=False)
+    with pytest.raises(G.GpuError) as e:
+        g.pages_reserve(pages, [0], [1])
+    assert e.value.code == -3 and int(pool.lens[0]) == length
+    g.debug_set_wait_limit(0)
+    assert call(wait=True)
+    o, a, most = attend64(q[:length], k, v, 0.1)
+    assert not bool(out[: rows - length].any())
+    assert float(((out[rows - length:].double() - o).abs() - attend_bound(o, a, most, "f16")).max()) <= 0
+    assert g.pages_reserve(pages, [0], [1]) and int(pool.lens[0]) == length + 1
+    g.close()
