@@ -773,7 +773,7 @@ attend_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ CUt
                         const int lo = from + edge * wk.x.per_block, hi = from + (wk.x.nb - edge + 1) * wk.x.per_block - 1;
                         int *mt = p.meta + cta * 8;
                         cuts = hi / per - (lo - 1) / per;
-                        mt[1] = wk.x.s.first + wk.x.tok0; mt[2] = wk.x.ntok; mt[3] = wk.x.h;
+                        mt[1] = wk.x.s.first + wk.x.tok0; mt[2] = wk.x.ntok; mt[3] = wk.x.h; mt[4] = !F32 && wk.x.ntok > tq;
                     }
                     ++n_seg;
                     more = wk.next(g);
@@ -1137,13 +1137,15 @@ __global__ void __launch_bounds__(256, 3) attend_join_kernel(const __grid_consta
     const int4 mt = *(const int4 *)(p.meta + blockIdx.x * 8);
     const int more = mt.x, row0 = mt.y, ntok = mt.z, h = mt.w;
     int odd = 0;
+    uint32_t bad = 0;   // rows of the warp that are not finite: bit iteration * ROWS + sub (four iterations at most: 32 rows or fewer a block)
     for (int i = threadIdx.x; i < p.n_ctas; i += 256) odd |= p.meta[i * 8 + 6];
     if (more > 0 && more < p.n_ctas - (int)blockIdx.x) {
         const int tq = 128 / a.group;
-        const bool wide = TY != PTY_F32 && ntok > tq;
+        const bool wide = p.meta[blockIdx.x * 8 + 4];
         const int n_rows = wide ? 128 + (ntok - tq) * a.group : ntok * a.group, sub = lane / LANES, ch = lane % LANES;
+        const int r_first = (blockIdx.y * 8 + warp) * ROWS, r_step = 8 * ROWS * gridDim.y;
 #pragma unroll 1
-        for (int r0 = (blockIdx.y * 8 + warp) * ROWS; r0 < n_rows; r0 += 8 * ROWS * gridDim.y) {
+        for (int r0 = r_first, it = 0; r0 < n_rows; r0 += r_step, it += ROWS) {
             const int r = min(r0 + sub, n_rows - 1), rr = r & 127, tok = (r >= 128 ? tq : 0) + rr / a.group;
             const bool mine = r0 + sub < n_rows && rr < tq * a.group;
             auto at = [&](int piece) { return (2 * ((int)blockIdx.x + piece) + (piece == 0)) * p.ws_rows + r; };
@@ -1182,11 +1184,14 @@ __global__ void __launch_bounds__(256, 3) attend_join_kernel(const __grid_consta
             o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
             const int row = row0 + tok, head = h * a.group + rr % a.group;
             if (mine) put4<TY>(a.out, row * a.os[0] + head * a.os[1] + ch * 4, o);
-            const uint32_t bad = __ballot_sync(~0u, mine && !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY));
+            const uint32_t is = __ballot_sync(~0u, mine && !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY));
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) bad |= (is >> (i * LANES) & (~0u >> (32 - LANES)) ? 1u : 0u) << (it + i);
+        }
 #pragma unroll 1
-            for (int i = 0; i < ROWS; ++i)
-                if (bad >> (i * LANES) & (~0u >> (32 - LANES)))
-                    attend_mend<D, T, C>(a, __shfl_sync(~0u, row, i * LANES), __shfl_sync(~0u, head, i * LANES), lane);
+        for (; bad; bad &= bad - 1) {
+            const int i = __ffs(bad) - 1, r = r_first + i / ROWS * r_step + i % ROWS, rr = r & 127;
+            attend_mend<D, T, C>(a, row0 + (r >= 128 ? tq : 0) + rr / a.group, h * a.group + rr % a.group, lane);
         }
     }
     if (__syncthreads_or(odd))
