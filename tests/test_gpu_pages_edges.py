@@ -199,3 +199,30 @@ def test_an_expired_wait_in_attention_is_reported_and_the_pool_lives_on(G):
     assert float(((out[rows - length:].double() - o).abs() - attend_bound(o, a, most, "f16")).max()) <= 0
     assert g.pages_reserve(pages, [0], [1]) and int(pool.lens[0]) == length + 1
     g.close()
+
+
+# ------------------------------------------------------------------------------------------------- the largest batch
+
+def test_a_step_of_as_many_sequences_as_a_batch_takes(G, g):
+    """4096 sequences, in any order: prompts of 1 to 40 rows, then a token each; every hundredth is held against 64 bits."""
+    n, page, dim, group = 4096, 8, 64, 2
+    rows = torch.randint(1, 41, (n,), generator=torch.Generator().manual_seed(80))
+    pool = Pool(1, int(((rows + 8) // page).sum()), page, 1, dim, "f16", n, 6, seed=80)
+    pages, r, order = G.KvPages(g, *pool.args()), gen(80), torch.randperm(n, generator=torch.Generator().manual_seed(81))
+    for step in (rows, torch.ones_like(rows)):
+        for part in order.split(1024):
+            assert g.pages_reserve(pages, part, step[part])
+        mine = step[order]
+        cu = torch.cat([torch.zeros(1, dtype=torch.int64), mine.cumsum(0)]).int().cuda()
+        total = int(mine.sum())
+        q, k, v = (torch.randn((total, h, dim), generator=r, device="cuda").half() for h in (group, 1, 1))
+        out, seqs = torch.empty_like(q), order.int().cuda()
+        assert g.rope_append(pages, 0, q, k, v, cu, None, seqs=seqs)
+        assert g.attend_pages(pages, 0, q, cu, dim ** -0.5, out, seqs=seqs, wait=True)
+        ends = cu.tolist()
+        for i in list(range(0, n, 100)) + [n - 1]:
+            part, (pk, pv) = slice(ends[i], ends[i + 1]), pool.read(int(order[i]))
+            assert torch.equal(pk[-int(mine[i]):], k[part]) and torch.equal(pv[-int(mine[i]):], v[part])
+            o, a, most = attend64(q[part], pk, pv, dim ** -0.5)
+            assert float(((out[part].double() - o).abs() - attend_bound(o, a, most, "f16")).max()) <= 0
+    assert pool.lens.tolist() == (rows + 1).tolist()
