@@ -98,16 +98,24 @@ __device__ __noinline__ void attend_row(const AttendParams &p, const SeqRows &s,
 // The maximum that the weights refer to moves only when a row's grows by more than 2^8 (LAZY): until then weights are at
 // most 2^8 (x 2^7 for f16, whose range is 2^-24 .. 2^16), and O keeps its scale.
 //
+// 16-bit rows: a weight is rounded to the rows' type, by half a step at most (f16 2^-11, bf16 2^-8, relative), because the
+// tensor instruction takes V and the weights in one type; maxima and the weights' sum stay in 32 bits and take the weight before
+// its rounding.  A second part, as below, would double the products with V and the weights' registers.  Against 64 bits the
+// results are off by 2.3e-4 to 2.9e-4 (f16; 2.1e-4 with weights in 32 bits, which is the result's own rounding) and 2.0e-3 to
+// 2.3e-3 (bf16; 1.7e-3).  O is summed over a CTA's whole range in TMEM, where sums are truncated at about 24 bits: with V = 1
+// everywhere most f16 results came out one step (2^-11) low over 2^20 positions a CTA, one in a thousand over 2^19, none over 2^17.
+//
 // 32-bit rows (over f16 pages): a query, scaled by a power of two of its own, and a weight are each the sum of two f16
 // values, 22 bits; every product is done for both.  The tensor cores' sums are truncated at about 24 bits, and over the
 // blocks of a long sequence that would add up to 2^-15: so O of a block starts from 0, and group 1 adds it to its registers
 // in 32 bits, while group 0 does the softmax of every block (tiles are narrow, two score and two O buffers).
 //
-// What bounds it, and what it measured.  Single tokens: the bytes of K and V; 64 sessions of 200 to 8192 positions (577 MB)
-// 107 us, 5.4 TB/s or 0.84 of the measured copy rate; one of 131077 positions 97 us, 0.86; the rest is 15 us of opening,
-// joining and cold code.  Chunks: a group's chain scores -> weights (1.1 us for 128 x 128: the exponentials alone are 0.6) ->
+// What bounds it, and what it measured (loops of single calls, from the best of several B200s to the slowest).  Single tokens:
+// the bytes of K and V; 64 sessions of 200 to 8192 positions (577 MB) 105 to 128 us, 4.5 to 5.5 TB/s or 0.70 to 0.85 of the
+// measured copy rate; one of 131077 positions 93 to 105 us, 0.79 to 0.89; the rest is 15 us of opening, joining and cold code.
+// Chunks: a group's chain scores -> weights (1.1 us for 128 x 128: the exponentials alone are 0.6) ->
 // both products (0.6) -> scores, with 0.5 us of hand-overs in between; two groups in turn keep the tensor cores half busy:
-// 4096 rows over 8192 positions 447 us, 920 TFLOP/s.  TMEM is full (two times 128 columns of scores and of O), so there is
+// 4096 rows over 8192 positions 444 to 496 us, 833 to 930 TFLOP/s.  TMEM is full (two times 128 columns of scores and of O), so there is
 // no third group and no second score buffer; 64-position steps with two of them took 600 us.
 // 32-bit rows: the tensor cores' time for every product done twice, 1.7 us a block.
 

@@ -512,7 +512,11 @@ int apk_rope_append(apk_ctx *ctx, const apk_rope_req *req, void *stream, int wai
  * sum_i softmax_i(scale * q.k_i) v_i over the positions i < lens with i <= p (causal != 0) and i > p - window
  * (window != 0); GQA group = n_heads / n_kv_heads <= 64, head_dim 64 or 128.  A row that sees no position
  * becomes zeros; rows that belong to no sequence are left alone.  What invisible positions hold
- * (infinities, NaN) does not matter.  Rows are of the pages' type, or f32 over f16 pages. */
+ * (infinities, NaN) does not matter, but where V is not finite the rows that meet it in their blocks of 128
+ * positions are done over one by one, which is slow.  Rows are of the pages' type, or f32 over f16
+ * pages; softmax weights of 16-bit rows are rounded to the rows' type (f32 rows: to 22 bits), sums and
+ * maxima are held in 32 bits.  Declined as too much for one call: (rows / (128 / group) + sequences) x
+ * (2 x width x page / 128 + 10) x kv heads of 2^30 and more (group: n_heads / n_kv_heads). */
 typedef struct {
     const apk_pages *pages;
     uint32_t layer;
