@@ -880,6 +880,8 @@ class Gpu:
                 ws_at = workspace.data_ptr()
         elif workspace.get_device() != dev:
             raise ValueError(f"workspace is on {workspace.device}")
+        elif not workspace.is_contiguous():
+            raise ValueError("workspace is not contiguous")
         else:
             ws_at, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         req = _ATTEND_REQ.pack(pages._p, layer, ty, q.data_ptr(), out.data_ptr(), q0, q1, o0, o1, heads, T, cu_at, seqs_at, n, scale,

@@ -255,6 +255,14 @@ def test_long_lists_that_are_refused(gpu, ctx):
             assert e.value.code == -1 and word in str(e.value) and str(dst[j]) in str(e.value)
 
 
+def test_a_workspace_that_is_not_what_its_size_says(gpu, ctx):
+    """An expanded tensor counts elements that it does not have."""
+    p, small = pool(gpu, ctx), Tensor(1 << 28, dtype="uint8", stride=(0,))
+    small.element_size = lambda: 1
+    with pytest.raises(ValueError):
+        attend(ctx, p, workspace=small)
+
+
 def test_null_requests_are_refused(gpu):
     lib, block = gpu.load_library(), C.create_string_buffer(1 << 16)
     h = C.addressof(block)
